@@ -4,6 +4,7 @@
 // (the unit the attention kernel fetches). A token's slot is page * page_size + offset; slots are 32-bit
 // (the host refuses caches of 2^31 tokens or more), every element offset is 64-bit.
 #include "common.cuh"
+#include <atomic>
 
 namespace {
 
@@ -18,7 +19,7 @@ namespace {
 // All or nothing: with too few free pages, a table too narrow, more tokens than slots or a negative length,
 // nothing is taken (table untouched, every slot -1, cu zero, total = cached) and used[1] says why.
 // Measured on the GPU: 3.7 us for a decode step of 256 requests, 4.1 us for 64 prompts of up to 2048 tokens.
-constexpr int PT_THREADS = 512;
+constexpr int PT_THREADS = 512, PT_MAX_REQUESTS = 8192;
 enum : int { PT_POOL = 1, PT_WIDTH = 2, PT_SLOTS = 4, PT_NEGATIVE = 8 };
 
 struct Pair {
@@ -245,12 +246,28 @@ struct PageTablesArgs {
   long long ld;
   int n_free, width, cap, B, shift, reserved;
 };
+// The kernel may take more than 48 KB of shared memory (its static part counts too, hence the KB less) once this has
+// been asked of the device; one limit for every call, so that no thread lowers another's.
+static int page_tables_prepared(int smem) {
+  constexpr int MAX_DEVICES = 64;
+  static std::atomic<bool> done[MAX_DEVICES];
+  if (smem <= 47 * 1024) return 0;
+  int dev = 0;
+  DT_CUDA_RET(cudaGetDevice(&dev));
+  if (dev >= MAX_DEVICES) return -12;
+  if (done[dev].load(std::memory_order_acquire)) return 0;
+  DT_CUDA_RET(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   3 * PT_MAX_REQUESTS * (int)sizeof(int)));
+  done[dev].store(true, std::memory_order_release);
+  return 0;
+}
 DT_API int dt_page_tables(const PageTablesArgs* args, cudaStream_t st) {
   const PageTablesArgs& a = *args;
-  if (a.B < 1 || a.B > 8192 || a.cap < 0 || a.n_free < 0 || a.width < 0 || a.shift < 0 || a.shift > 16) return -10;
+  if (a.B < 1 || a.B > PT_MAX_REQUESTS || a.cap < 0 || a.n_free < 0 || a.width < 0 || a.shift < 0 || a.shift > 16)
+    return -10;
   const int smem = 3 * a.B * (int)sizeof(int);
-  if (smem > 48 * 1024)
-    DT_CUDA_RET(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int rc = page_tables_prepared(smem);
+  if (rc) return rc;
   const int work = a.cap > a.B ? a.cap : a.B;
   int grid = (work + 2 * PT_THREADS - 1) / (2 * PT_THREADS);
   if (grid > 148) grid = 148;
