@@ -30,9 +30,17 @@ enum DtError : int {
 // Defined once in errors.cu.
 extern __device__ int dt_error_word;
 extern __device__ int dt_error_site;
+extern __device__ int dt_report_word;
+extern __device__ int dt_report_site;
 
 __device__ __forceinline__ void dt_set_error(int code, int site) {
   if (atomicCAS(&dt_error_word, 0, code) == 0) dt_error_site = site;
+}
+// A bad value in one caller's data (a page id, a slot, a length), which the kernel has left out. It is read and cleared
+// with the error word, but in a word of its own: every bounded wait gives up while dt_error_word is set, and what one
+// caller passes must not end the work of others, nor keep a later time-out from being recorded.
+__device__ __forceinline__ void dt_report(int code, int site) {
+  if (atomicCAS(&dt_report_word, 0, code) == 0) dt_report_site = site;
 }
 
 __device__ __forceinline__ uint64_t dt_globaltimer() {

@@ -202,7 +202,7 @@ kv_append_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld, const floa
     const int page = slot[k] >> shift;
     if (slot[k] < 0) continue;
     if (page >= num_pages || pos[k] < 0 || pos[k] >= max_pos) {
-      dt_set_error(DT_ERR_BOUNDS, 700);
+      dt_report(DT_ERR_BOUNDS, 700);
       continue;
     }
     __nv_bfloat16* dst;

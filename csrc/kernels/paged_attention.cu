@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PlanArgs
   if (empty) atomicAdd(&s_empty, empty);
   __syncthreads();
   if (tid == 0) {
-    if (status) dt_set_error(DT_ERR_BAD_ARG, 710 + status);
+    if (status) dt_report(DT_ERR_BAD_ARG, 710 + status);
     plan[H_MAGIC] = PLAN_MAGIC;
     plan[H_STATUS] = status;
     plan[H_B] = a.B;
@@ -494,7 +494,7 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (!a.wide_first) pdl_wait();  // the plan, and the cache and queries that the kernels before it wrote (see AttnArgs)
   pdl_next();
   if (!head.load(a, D)) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) dt_set_error(DT_ERR_BAD_ARG, 721);
+    if (threadIdx.x == 0 && blockIdx.x == 0) dt_report(DT_ERR_BAD_ARG, 721);
     pdl_wait();
     return;
   }
@@ -524,7 +524,7 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       p += lane;
       int id = p * P < f.keys ? __ldcg(table_of(f) + p) : 0;
       if (p * P < f.keys && (unsigned)id >= (unsigned)a.pages) {
-        dt_set_error(DT_ERR_BOUNDS, 723);
+        dt_report(DT_ERR_BOUNDS, 723);
         id = -1;
       }
       return id;
@@ -960,7 +960,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (a.wide_first) pdl_wait();
   pdl_next();
   if (!head.load(a, D)) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) dt_set_error(DT_ERR_BAD_ARG, 741);
+    if (threadIdx.x == 0 && blockIdx.x == 0) dt_report(DT_ERR_BAD_ARG, 741);
     pdl_wait();
     return;
   }
@@ -1073,7 +1073,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const int p = win0 + lane;
             win = p * P < en.keys ? __ldcg(table + p) : 0;
             if (p * P < en.keys && (unsigned)win >= (unsigned)a.pages) {
-              dt_set_error(DT_ERR_BOUNDS, 743);
+              dt_report(DT_ERR_BOUNDS, 743);
               win = -1;
             }
           }

@@ -9,9 +9,11 @@ One step of a batch, all on the GPU and fit for capture in a CUDA graph (every b
     per layer: kv_append(...) bias + rotation of the QKV rows, K and V into their slots
                paged_attention(...) queries over the pages, shared prefixes computed once for their group
 
-Calls check types, shapes and devices and raise ``ValueError``; what only the GPU can see (a table entry
-outside the cache, a position outside the rotation tables) is skipped there and recorded in the library's
-device error word (``ops.device_error``).
+Calls check types, shapes and devices and raise ``ValueError``. What only the GPU can see is reported through
+``ops.device_error`` and touches no other request: the append leaves out a row whose slot or position is none, the
+attention takes keys and values on a page outside the cache as zeros (their request's rows are then meaningless), and
+lengths that contradict each other leave the step without work. Such a report stays until ``ops.clear_device_error``;
+it stops no other call.
 
 A decode step's calls take a few microseconds on the GPU, so what they cost here counts: each call tests its
 arguments in one expression and only names what is wrong once that has failed, and the launchers take one packed
@@ -182,7 +184,7 @@ def kv_append(qkv, bias, cos, sin, slots, positions, q, k_cache, v_cache, *, str
     or None, ``cos`` / ``sin`` [max_pos, d/2] fp32 tables of the rotate-half form. Row t with slot ``slots[t]``
     >= 0: ``q[t]`` = rot(q + bias), K row = rot(k + bias), V row = v + bias, each rounded once to bf16; a row
     with a negative slot is left out (its ``q`` row too). Two rows of one call must not have the same slot.
-    A slot outside the cache or a position outside the tables leaves its row out and sets the device error."""
+    A slot outside the cache or a position outside the tables leaves its row out and is reported."""
     pages, nkv, page_size, d = _cache(k_cache, v_cache)
     rows, qs, cs = qkv.shape, q.shape, cos.shape
     if d % 16 or d < 16:
@@ -264,7 +266,7 @@ class AttentionPlan:
         ``prefix_lens`` [G], ``cu_group`` [G+1]): group y, requests ``cu_group[y] .. cu_group[y+1]``, has
         ``prefix_lens[y]`` keys in front of every request's own (``cu_group`` covers all requests). The tensors
         must stay unchanged until the step's last ``paged_attention`` has run. Lengths that contradict each
-        other or the tables set the device error and leave the step without work."""
+        other or the tables are reported and leave the step without work."""
         B, G = self.B, self.G
         ts = tables.shape
         if not (cu_q.shape == (B + 1,) and lens.shape == (B,) and len(ts) == 2 and ts[0] == B and cu_q.dtype is _I32 and

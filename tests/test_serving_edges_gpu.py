@@ -45,3 +45,81 @@ def test_page_tables_of_4096_requests_before_any_larger_call():
 @pytest.mark.parametrize("B", [4073, 4074, 4096, 4097, 8192, 5000])
 def test_page_tables_of_many_requests(B):
     _decode_tables(B)
+
+
+# ───────────────────────── one caller's bad data ─────────────────────────
+def _long_calls():
+    """Attention of both kernels and a GEMM, whose waits poll many times: (run, outputs)."""
+    from distrain_b200 import ops
+    from test_paged_gpu import Batch
+    batches = [Batch([1] * 64, [4096 - 37 * i for i in range(64)], 16, 4, 128, 64, seed=3),
+               Batch([900, 1, 300], [2000, 3000, 300], 16, 4, 128, 64, seed=4)]
+    g = torch.Generator(device=DEV).manual_seed(0)
+    a, b = (torch.randn(4096, 4096, generator=g, device=DEV).bfloat16() for _ in range(2))
+
+    def run():
+        c = torch.full((4096, 4096), 7.0, device=DEV)
+        out = [x.run() for x in batches]
+        ops.gemm(a, b, c, M=4096, N=4096, K=4096)
+        return out + [c]
+    return run
+
+
+@pytest.mark.parametrize("what", ["slot", "page", "lengths"])
+def test_a_report_stops_no_other_call(what):
+    """Bad data stays reported until it is cleared; the calls after it (and beside it) give what they gave before."""
+    from distrain_b200 import ops
+    from distrain_b200.ops import paged
+    from test_paged_gpu import Batch
+    ops.clear_device_error()
+    run = _long_calls()
+    want = run()
+    assert ops.device_error() == (0, 0)
+    if what == "slot":
+        d, P = 32, 16
+        cos = torch.ones(8, d // 2, device=DEV)
+        kc, vc = (torch.zeros(2, 2, P, d, device=DEV).bfloat16() for _ in range(2))
+        q = torch.zeros(1, 4 * d, device=DEV).bfloat16()
+        paged.kv_append(torch.ones(1, 8 * d, device=DEV).bfloat16(), None, cos, cos, _i([2 * P]), _i([0]), q, kc, vc)
+        code = 5
+    else:
+        b = Batch([1, 1], [50, 20], 4, 2, 64, 16)
+        if what == "page":
+            b.tables[0, 1] = 10 ** 6
+        else:
+            b.len_t[1] = 10 ** 6
+        b.run()
+        code = 5 if what == "page" else 6
+    assert ops.device_error()[0] == code
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(want, run()))
+    assert ops.device_error()[0] == code  # still there
+    ops.clear_device_error()
+    assert ops.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [50, 20, 90]), ([40, 30, 1], [50, 70, 90])])
+@pytest.mark.parametrize("where", ["own", "prefix"])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+def test_a_bad_page_touches_its_request_alone(new, lens, where, bad):
+    """Keys and values on a page outside the cache count as zeros; the other requests' rows are the same bits."""
+    from distrain_b200 import ops
+    from test_paged_gpu import Batch
+    ops.clear_device_error()
+    b = Batch(new, lens, 4, 2, 64, 16, pre=[40, 70], sizes=[1, 2], seed=2)
+    clean = b.run()
+    if where == "own":
+        b.tables[0, 1] = bad
+        b.ks[0][:, 16:32] = 0
+        b.vs[0][:, 16:32] = 0
+    else:
+        b.prefix[0][0, 1] = bad
+        b.pks[0][:, 16:32] = 0
+        b.pvs[0][:, 16:32] = 0
+    out = b.run()
+    assert ops.device_error()[0] == 5
+    ops.clear_device_error()
+    assert torch.equal(out[new[0]:], clean[new[0]:])
+    ref, size, _ = b.ref()
+    # (the bound of an attention output: test_paged_gpu.py)
+    assert ((out.double().view(ref.shape) - ref).abs() <= ref.abs() * 2 ** -8 + (2 ** -7 + 2 ** -13) * size + 1e-30).all()
