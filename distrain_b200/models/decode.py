@@ -107,11 +107,18 @@ class PagedDecoder:
         ops.gemm(a, e.E16, out, M=M, N=e.V, K=e.H, ldc=self.ldv)
         return out[:n, :e.V]
 
+    def _known(self, ids: Sequence[int]):
+        """Refuses what is no token id: the embedding's rows are read without a bound."""
+        for t in ids:
+            if not 0 <= t < self.eng.V:
+                raise ValueError(f"token id {t} outside the vocabulary of {self.eng.V}")
+
     def prefill(self, ids: Sequence[int]) -> torch.Tensor:
         """Forward of a prompt into fresh pages; fp32 logits [1, V] of the token after it."""
         T = len(ids)
         if not 1 <= T <= self.max_prompt:
             raise ValueError(f"prompt of {T} tokens: 1 to {self.max_prompt}")
+        self._known(ids)
         e, M = self.eng, _pad(T, ROWS)
         b = self._buffers(M)
         b["ids"].zero_()
@@ -150,6 +157,7 @@ class PagedDecoder:
             raise ValueError(f"{len(tokens)} tokens for {self.n} answers")
         if self.length >= self.max_new:
             raise ValueError(f"answers have {self.max_new} tokens, the most there is room for")
+        self._known(tokens)
         b = self._buffers(self.rows)
         b["ids"][:self.n] = torch.tensor(tokens, dtype=torch.int32)
         self._tables(b, self.cached, self.one, self.tables, self.cu, self.total, self.start,
