@@ -2,9 +2,10 @@
 
 ``PagedDecoder`` runs the model of a (forward-only) ``TrainEngine`` on its weights. ``prefill`` computes a
 prompt and leaves its keys and values in pages; ``branch(n)`` makes those pages the shared prefix of n answers;
-``step`` adds one token to each of them. Lengths, page tables, slots and the attention's work list are made on
-the GPU each step (``ops.paged``); per layer the QKV GEMM is followed by the append (bias, rotation, K and V to
-their slots) and the attention, in which the prompt's keys are read once for all answers.
+``step`` adds one token to each of them; ``check`` says whether the GPU could do it all. Lengths, page tables, slots
+and the attention's work list are made on the GPU each step (``ops.paged``); per layer the QKV GEMM is followed by the
+append (bias, rotation, K and V to their slots) and the attention, in which the prompt's keys are read once for all
+answers.
 
 The reference re-runs the whole forward for every new token (node/cli/src/main.rs:1416-1548); this computes the
 same logits from the new tokens alone.
@@ -46,7 +47,8 @@ class PagedDecoder:
         self.ldv = _pad(eng.V, 8)
         self._bufs = {}
         self.taken = 0  # pages in use
-        self.prompt_len = self.n = 0
+        self.used = self._ints(self.max_new + 1, 2)  # what page_tables said of the prompt (row 0) and of each step
+        self.prompt_len = self.n = self.length = 0
 
     def _ints(self, *shape):
         return torch.zeros(*shape, dtype=torch.int32, device=self.dev)
@@ -63,11 +65,10 @@ class PagedDecoder:
                                   h=new(M, e.F))}
         return self._bufs[M]
 
-    def _tables(self, b, cached, new, tables, cu, total, start, pages):
+    def _tables(self, b, cached, new, tables, cu, total, start, pages, row):
         """Page tables of a step whose requests take ``pages`` pages together (the host knows all lengths)."""
-        used = self._ints(2)
-        paged.page_tables(cached, new, self.free[self.taken:], tables, b["slots"], b["positions"], cu, total, used,
-                          page_size=self.P, start=start)
+        paged.page_tables(cached, new, self.free[self.taken:], tables, b["slots"], b["positions"], cu, total,
+                          self.used[row], page_size=self.P, start=start)
         self.taken += pages
 
     def _forward(self, b, M: int, plan):
@@ -126,11 +127,11 @@ class PagedDecoder:
         self.taken = 0
         self.prefix = torch.full((1, self.prompt_pages), -1, dtype=torch.int32, device=self.dev)
         cu, total = self._ints(2), self._ints(1)
-        self._tables(b, self._ints(1), torch.full_like(total, T), self.prefix, cu, total, None, -(-T // self.P))
+        self._tables(b, self._ints(1), torch.full_like(total, T), self.prefix, cu, total, None, -(-T // self.P), 0)
         plan = paged.AttentionPlan(M, 1, nh=e.nh, nkv=e.nkv, d=e.d, page_size=self.P, device=self.dev)
         plan.build(cu, total, self.prefix)
         hidden = self._forward(b, M, plan)
-        self.prompt_len, self.n = T, 0
+        self.prompt_len, self.n, self.length = T, 0, 0
         return self._logits(hidden[T - 1:T])
 
     def branch(self, n: int):
@@ -151,6 +152,17 @@ class PagedDecoder:
         self.rows = _pad(n, ROWS)
         self.plan = paged.AttentionPlan(self.rows, n, 1, nh=e.nh, nkv=e.nkv, d=e.d, page_size=self.P, device=self.dev)
 
+    def check(self):
+        """Raises if the GPU could not do what the steps since ``prefill`` asked for; their logits are worth nothing then.
+        Waits for the GPU: once at the end of an answer is enough. The library's error state is clear afterwards."""
+        code, site = ops.device_error()
+        if code:
+            ops.clear_device_error()
+            raise RuntimeError(f"generation failed on the GPU: error {code} at site {site}")
+        refused = self.used[:self.length + 1, 1].amax().item()
+        if refused:
+            raise RuntimeError(f"generation failed on the GPU: page tables refused a step ({refused})")
+
     def step(self, tokens: List[int]) -> torch.Tensor:
         """Adds ``tokens[i]`` to answer i; fp32 logits [n, V] of the tokens after them."""
         if len(tokens) != self.n or self.n == 0:
@@ -161,7 +173,7 @@ class PagedDecoder:
         b = self._buffers(self.rows)
         b["ids"][:self.n] = torch.tensor(tokens, dtype=torch.int32)
         self._tables(b, self.cached, self.one, self.tables, self.cu, self.total, self.start,
-                     self.n if self.length % self.P == 0 else 0)
+                     self.n if self.length % self.P == 0 else 0, self.length + 1)
         self.plan.build(self.cu, self.total, self.tables, prefix=self.group)
         hidden = self._forward(b, self.rows, self.plan)
         self.cached.add_(self.one)

@@ -169,7 +169,7 @@ def sample_cached(dec, ids: List[int], n: int, max_tokens: int, temperature: flo
                   options: Optional[LogitOptions] = None) -> List[Tuple[List[int], str]]:
     """n answers of up to ``max_tokens`` tokens to one prompt through a ``PagedDecoder``: (new tokens, finish
     reason) of each, drawn like ``sample`` with seeds ``seed``, ``seed + 1``, .... A prompt that leaves too little
-    room loses tokens on the left."""
+    room loses tokens on the left. Raises if the GPU reports that a step could not be done."""
     ids = (list(ids) if ids else [1])[-dec.max_prompt:]
     if max_tokens <= 0:
         return [([], "length") for _ in range(n)]
@@ -186,32 +186,35 @@ def sample_cached(dec, ids: List[int], n: int, max_tokens: int, temperature: flo
         prompt = torch.full((n,), len(ids), dtype=torch.int32, device=dev)
         lens = prompt.clone()
         args = options.device_args(n, history, lens, prompt, V)
-    logits = dec.prefill(ids).expand(n, V)  # every answer's first token comes from the prompt's last position
-    for k in range(int(max_tokens)):
-        if k:
-            if k == 1:
-                dec.branch(n)
-            logits = dec.step([o[-1] for o in out])
-        if args is not None:
-            z = torch.empty(n, V, dtype=torch.float32, device=dev)
-            process_logits(logits, z, **args)
-        else:
-            z = logits
-        if temperature <= 0:
-            tokens = z.argmax(-1).tolist()
-        else:
-            z = z.cpu()
-            tokens = [_draw(z[i], temperature, gens[i]) if i in running else out[i][-1] for i in range(n)]
-        for i in list(running):
-            out[i].append(int(tokens[i]))
-            if (stop_token is not None and out[i][-1] == stop_token) or (stop_fn is not None and stop_fn(out[i])):
-                reason[i] = "stop"
-                running.remove(i)
-        if not running:
-            break
-        if args is not None:  # (an answer that has stopped keeps its last token; its logits are not used)
-            history[:, len(ids) + k] = torch.tensor([o[-1] for o in out], dtype=torch.int32)
-            lens.add_(1)
+    try:
+        logits = dec.prefill(ids).expand(n, V)  # every answer's first token comes from the prompt's last position
+        for k in range(int(max_tokens)):
+            if k:
+                if k == 1:
+                    dec.branch(n)
+                logits = dec.step([o[-1] for o in out])
+            if args is not None:
+                z = torch.empty(n, V, dtype=torch.float32, device=dev)
+                process_logits(logits, z, **args)
+            else:
+                z = logits
+            if temperature <= 0:
+                tokens = z.argmax(-1).tolist()
+            else:
+                z = z.cpu()
+                tokens = [_draw(z[i], temperature, gens[i]) if i in running else out[i][-1] for i in range(n)]
+            for i in list(running):
+                out[i].append(int(tokens[i]))
+                if (stop_token is not None and out[i][-1] == stop_token) or (stop_fn is not None and stop_fn(out[i])):
+                    reason[i] = "stop"
+                    running.remove(i)
+            if not running:
+                break
+            if args is not None:  # (an answer that has stopped keeps its last token; its logits are not used)
+                history[:, len(ids) + k] = torch.tensor([o[-1] for o in out], dtype=torch.int32)
+                lens.add_(1)
+    finally:
+        dec.check()  # (a wait given up or a step refused makes wrong tokens, and maybe an exception after them)
     return list(zip(out, reason))
 
 

@@ -25,3 +25,51 @@ def test_ids_outside_the_vocabulary_are_refused(bad):
         dec.step([99, bad])
     with pytest.raises(AttributeError):  # ids of the vocabulary pass
         dec.prefill([0, 99])
+
+
+class FakeDecoder:
+    """Logits of a fixed table instead of a model: the token after t is drawn from row t. Takes part in
+    ``sample_cached`` without a GPU."""
+
+    def __init__(self, V=50, max_prompt=16, max_batch=4, report=None, seed=0):
+        self.eng, self.dev, self.max_prompt, self.max_batch = SimpleNamespace(V=V), torch.device("cpu"), max_prompt, max_batch
+        self.z = torch.randn(V, V, generator=torch.Generator().manual_seed(seed))
+        self.report, self.checked, self.n = report, 0, 0
+
+    def prefill(self, ids):
+        return self.z[ids[-1]:ids[-1] + 1]
+
+    def branch(self, n):
+        assert 1 <= n <= self.max_batch
+        self.n = n
+
+    def step(self, tokens):
+        assert len(tokens) == self.n
+        return self.z[torch.tensor(tokens)]
+
+    def check(self):
+        self.checked += 1
+        if self.report:
+            raise RuntimeError(self.report)
+
+
+def test_what_the_gpu_reports_fails_the_request():
+    from distrain_b200.serve import sample_cached
+    dec = FakeDecoder()
+    assert len(sample_cached(dec, [1, 2], 2, 5)[0][0]) == 5 and dec.checked == 1
+    for tokens in (1, 5):
+        with pytest.raises(RuntimeError, match="gave up"):
+            sample_cached(FakeDecoder(report="gave up"), [1, 2], 1, tokens)
+    first = sample_cached(dec, [1, 2], 1, 1)[0][0][0]
+    with pytest.raises(RuntimeError, match="gave up"):  # an answer that stops is checked too
+        sample_cached(FakeDecoder(report="gave up"), [1, 2], 1, 5, stop_token=first)
+
+
+def test_a_request_that_ends_in_an_exception_is_checked_too():
+    """The report must not be left for the next request to find."""
+    from distrain_b200.serve import sample_cached
+    dec = FakeDecoder()
+    dec.z[:] = float("nan")
+    with pytest.raises(RuntimeError, match="nan"):
+        sample_cached(dec, [1, 2], 1, 3, temperature=1.0)
+    assert dec.checked == 1

@@ -123,3 +123,32 @@ def test_a_bad_page_touches_its_request_alone(new, lens, where, bad):
     ref, size, _ = b.ref()
     # (the bound of an attention output: test_paged_gpu.py)
     assert ((out.double().view(ref.shape) - ref).abs() <= ref.abs() * 2 ** -8 + (2 ** -7 + 2 ** -13) * size + 1e-30).all()
+
+
+# ───────────────────────── generation ─────────────────────────
+def test_generation_fails_on_what_the_gpu_reports():
+    """A page lost from a decoder's tables, a step its page tables refuse, and a request after each that is as before."""
+    from distrain_b200 import ops
+    from distrain_b200.serve import sample_cached
+    from test_decode_gpu import _decoder
+    ops.clear_device_error()
+    _, _, dec = _decoder()
+    ids = [3, 5, 7, 11, 13] * 9
+    want = sample_cached(dec, ids, 2, 20)
+    branch = dec.branch
+
+    def lost(n):
+        branch(n)
+        dec.prefix[0, 1] = 10 ** 6
+
+    def full(n):
+        branch(n)
+        dec.cached += 16 * dec.answer_pages  # a table row has no room behind these
+
+    for bad, what, tokens in ((lost, "error 5", 20), (full, "page tables", 2)):
+        dec.branch = bad
+        with pytest.raises(RuntimeError, match=what):
+            sample_cached(dec, ids, 2, tokens)
+        dec.branch = branch
+        assert ops.device_error() == (0, 0)
+        assert sample_cached(dec, ids, 2, 20) == want
