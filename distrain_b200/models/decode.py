@@ -120,6 +120,7 @@ class PagedDecoder:
         if not 1 <= T <= self.max_prompt:
             raise ValueError(f"prompt of {T} tokens: 1 to {self.max_prompt}")
         self._known(ids)
+        self.prompt_len = self.n = self.length = 0  # (the pages change from here on: a failure leaves no prompt to continue)
         e, M = self.eng, _pad(T, ROWS)
         b = self._buffers(M)
         b["ids"].zero_()
@@ -131,7 +132,7 @@ class PagedDecoder:
         plan = paged.AttentionPlan(M, 1, nh=e.nh, nkv=e.nkv, d=e.d, page_size=self.P, device=self.dev)
         plan.build(cu, total, self.prefix)
         hidden = self._forward(b, M, plan)
-        self.prompt_len, self.n, self.length = T, 0, 0
+        self.prompt_len = T
         return self._logits(hidden[T - 1:T])
 
     def branch(self, n: int):
@@ -141,7 +142,7 @@ class PagedDecoder:
         if not 1 <= n <= self.max_batch:
             raise ValueError(f"{n} answers: 1 to {self.max_batch}")
         e = self.eng
-        self.n, self.length = n, 0
+        self.n = self.length = 0  # (until the buffers below are those of n answers)
         self.taken = -(-self.prompt_len // self.P)
         self.tables = torch.full((n, self.answer_pages), -1, dtype=torch.int32, device=self.dev)
         self.cached, self.one = self._ints(n), torch.ones(n, dtype=torch.int32, device=self.dev)
@@ -151,6 +152,7 @@ class PagedDecoder:
                       torch.tensor([0, n], dtype=torch.int32, device=self.dev))
         self.rows = _pad(n, ROWS)
         self.plan = paged.AttentionPlan(self.rows, n, 1, nh=e.nh, nkv=e.nkv, d=e.d, page_size=self.P, device=self.dev)
+        self.n = n
 
     def check(self):
         """Raises if the GPU could not do what the steps since ``prefill`` asked for; their logits are worth nothing then.

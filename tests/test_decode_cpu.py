@@ -73,3 +73,26 @@ def test_a_request_that_ends_in_an_exception_is_checked_too():
     with pytest.raises(RuntimeError, match="nan"):
         sample_cached(dec, [1, 2], 1, 3, temperature=1.0)
     assert dec.checked == 1
+
+
+def test_a_prompt_that_fails_leaves_nothing_to_continue():
+    """The pages of the prompt before are overwritten by then."""
+    dec = _decoder(prompt_len=5)
+    with pytest.raises(AttributeError):  # fails behind the checks
+        dec.prefill([1, 2])
+    with pytest.raises(RuntimeError, match="prefill"):
+        dec.branch(1)
+    with pytest.raises(ValueError, match="tokens"):
+        dec.step([1, 2])
+    dec = _decoder(prompt_len=5)
+    with pytest.raises(ValueError):  # a refused prompt changes nothing
+        dec.prefill([])
+    assert (dec.prompt_len, dec.n) == (5, 2)
+
+
+def test_answers_whose_buffers_fail_cannot_be_stepped():
+    dec = _decoder(prompt_len=5)
+    with pytest.raises(AttributeError):
+        dec.branch(1)
+    with pytest.raises(ValueError, match="tokens"):
+        dec.step([1])
