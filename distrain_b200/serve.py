@@ -26,7 +26,6 @@ from __future__ import annotations
 
 import ctypes
 import json
-import math
 import threading
 import time
 import uuid
@@ -87,6 +86,13 @@ class EngineLM:
             return (xs[len(ctx) - 1:len(ctx)].float() @ eng.E.t())[0].cpu()
 
 
+def whole(v) -> int:
+    """``v`` as a whole number; ValueError for a number that is none (1.7, infinity)."""
+    if isinstance(v, float) and not v.is_integer():
+        raise ValueError(f"{v} is not a whole number")
+    return int(v)
+
+
 @dataclass
 class LogitOptions:
     """What a request changes in the logits before a token is drawn (``ops.sampling.process_logits``)."""
@@ -97,28 +103,33 @@ class LogitOptions:
     allowed: Optional[List[int]] = None
 
     MAX_BIAS = 1024  # entries of a logit_bias
+    # Of penalties and biases, and of the repetition penalty and its reciprocal: products with counts and sums with logits
+    # stay far inside fp32, where an overflow would make NaN of tokens that no penalty is meant for.
+    LIMIT = 1e9
+
+    def __post_init__(self):
+        for name, v in [("presence", self.presence), ("frequency", self.frequency)] + \
+                [(f"bias of token {t}", b) for t, b in self.bias.items()]:
+            if not abs(v) <= self.LIMIT:
+                raise ValueError(f"{name}: {v} is not in [-{self.LIMIT:g}, {self.LIMIT:g}]")
+        if not 1 / self.LIMIT <= self.repetition <= self.LIMIT:
+            raise ValueError(f"repetition: {self.repetition} is not in [{1 / self.LIMIT:g}, {self.LIMIT:g}]")
 
     @classmethod
     def from_request(cls, req: dict, vocab: int) -> Optional["LogitOptions"]:
         """The options of a request; None if it has none of them. ValueError for what makes no sense."""
         def number(key, default):
             v = req.get(key)
-            v = default if v is None else float(v)
-            if not math.isfinite(v):
-                raise ValueError(f"{key} must be finite")
-            return v
+            return default if v is None else float(v)
         try:
-            o = cls(number("presence_penalty", 0.0), number("frequency_penalty", 0.0), number("repetition_penalty", 1.0))
-            o.bias = {int(k): float(v) for k, v in (req.get("logit_bias") or {}).items()}
             allowed = req.get("allowed_token_ids")
-            o.allowed = None if allowed is None else sorted({int(t) for t in allowed})
-        except (TypeError, AttributeError) as e:
+            o = cls(number("presence_penalty", 0.0), number("frequency_penalty", 0.0), number("repetition_penalty", 1.0),
+                    {whole(k): float(v) for k, v in (req.get("logit_bias") or {}).items()},
+                    None if allowed is None else sorted({whole(t) for t in allowed}))
+        except (TypeError, AttributeError, OverflowError) as e:
             raise ValueError(f"penalties are numbers, logit_bias an object, allowed_token_ids a list: {e}")
-        if o.repetition <= 0:
-            raise ValueError("repetition_penalty must be positive")
-        if len(o.bias) > cls.MAX_BIAS or any(not 0 <= t < vocab for t in o.bias) or \
-                not all(math.isfinite(v) for v in o.bias.values()):
-            raise ValueError(f"logit_bias: at most {cls.MAX_BIAS} token ids of the vocabulary with finite biases")
+        if len(o.bias) > cls.MAX_BIAS or any(not 0 <= t < vocab for t in o.bias):
+            raise ValueError(f"logit_bias: at most {cls.MAX_BIAS} token ids of the vocabulary")
         if o.allowed is not None and (not o.allowed or o.allowed[0] < 0 or o.allowed[-1] >= vocab):
             raise ValueError("allowed_token_ids: one or more token ids of the vocabulary")
         return None if o == cls() else o

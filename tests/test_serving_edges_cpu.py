@@ -1,0 +1,67 @@
+"""Completion requests at the edges of what the server accepts, on the CPU."""
+import json
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def srv(tmp_path_factory):
+    from distrain_b200.config import ModelConfig
+    from distrain_b200.models.params import ParamLayout, init_flat
+    from distrain_b200.serve import CompletionServer
+    from distrain_b200.utils.checkpoint import save_safetensors
+    cfg = ModelConfig(hidden_dim=32, num_layers=2, num_heads=4, num_kv_heads=2, ffn_hidden_dim=64, vocab_size=260,
+                      max_seq_len=128, rope_theta=10000.0)
+    L = ParamLayout(cfg)
+    path = str(tmp_path_factory.mktemp("ckpt") / "m.safetensors")
+    save_safetensors(L.to_state_dict(init_flat(L, seed=3)), path)
+    return CompletionServer(path, "cpu", tokenizer="bytes", max_tokens_cap=16, max_n=3)
+
+
+def _post(srv, body, route="/v1/completions"):
+    base = {"prompt": [1, 2, 3], "messages": [{"role": "user", "content": "hi"}], "max_tokens": 4}
+    text = json.dumps(dict(base, **body)) if isinstance(body, dict) else body
+    return srv.handle_request("POST", route, text.encode())
+
+
+@pytest.mark.parametrize("route", ["/v1/completions", "/v1/chat/completions"])
+@pytest.mark.parametrize("body", [
+    # beyond fp32, where the product with a count of zero is NaN for every other token
+    {"presence_penalty": 1e39}, {"frequency_penalty": 1e39}, {"frequency_penalty": -1e39}, {"logit_bias": {"7": 1e39}},
+    {"logit_bias": {"7": -1e300}}, {"repetition_penalty": 1e39},
+    # zero in fp32, or a reciprocal beyond it
+    {"repetition_penalty": 1e-50}, {"repetition_penalty": 1e-39},
+    # beyond doubles
+    {"presence_penalty": 10 ** 400}, {"frequency_penalty": 10 ** 400}, {"logit_bias": {"7": 10 ** 400}},
+    {"allowed_token_ids": [float("inf")]}, {"allowed_token_ids": [float("nan")]}, {"allowed_token_ids": [10 ** 400]},
+    {"presence_penalty": float("nan")}, {"logit_bias": {"7": float("nan")}},
+    # not a token id
+    {"allowed_token_ids": [1.7]}, {"logit_bias": {"1.7": 1}}])
+def test_options_past_the_edge_of_fp32_are_refused(srv, route, body):
+    st, out = _post(srv, body, route)
+    assert st == 400 and out["error"]["type"] == "invalid_request_error", out
+
+
+@pytest.mark.parametrize("body", [
+    {"presence_penalty": 1e9}, {"presence_penalty": -1e9}, {"frequency_penalty": 1e9}, {"frequency_penalty": -1e9},
+    {"repetition_penalty": 1e9}, {"repetition_penalty": 1e-9}, {"logit_bias": {"7": 1e9}}, {"logit_bias": {"7": -1e9}},
+    {"presence_penalty": 1e9, "frequency_penalty": 1e9, "repetition_penalty": 1e9, "logit_bias": {"7": 1e9}},
+    {"allowed_token_ids": [1.0, 2]}])
+@pytest.mark.parametrize("temperature", [0, 1.0])
+def test_options_at_their_limits_work(srv, body, temperature):
+    from distrain_b200.serve import LogitOptions
+    st, out = _post(srv, dict(body, temperature=temperature))
+    assert st == 200 and len(out["choices"][0]["token_ids"]) == 4, out
+    o = LogitOptions.from_request(body, 260)
+    z = o.apply(torch.linspace(-20, 20, 260), [1, 2, 2, 3, 7], 2)
+    assert not torch.isnan(z).any() and (z < float("inf")).all()
+    if "allowed_token_ids" in body:
+        assert o.allowed == [1, 2]
+
+
+def test_options_made_in_python_are_checked_too():
+    from distrain_b200.serve import LogitOptions
+    for kw in (dict(presence=1e39), dict(frequency=float("inf")), dict(repetition=0.0), dict(bias={3: float("nan")})):
+        with pytest.raises(ValueError):
+            LogitOptions(**kw)
