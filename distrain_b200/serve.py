@@ -12,9 +12,10 @@ once into a paged key/value cache and every step computes the new tokens alone (
 ``n`` answers of a request then share the prompt's pages.
 
 Routes: ``POST /v1/completions`` with {"prompt": text or [token ids], "max_tokens", "temperature",
-"seed", "stop_token", "n", "presence_penalty", "frequency_penalty", "repetition_penalty", "logit_bias":
-{token id: bias}, "allowed_token_ids"} -> {"id", "object": "text_completion", "created", "model", "choices": [{"text",
-"token_ids", "index", "finish_reason"}], "usage": {"prompt_tokens", "completion_tokens",
+"seed", "stop_token", "n" (a whole number up to ``max_n``), "presence_penalty", "frequency_penalty",
+"repetition_penalty", "logit_bias": {token id: bias}, "allowed_token_ids"; of these a null field is not there, and one
+that is no such value or out of range is a 400 (``LogitOptions``)} -> {"id", "object": "text_completion", "created",
+"model", "choices": [{"text", "token_ids", "index", "finish_reason"}], "usage": {"prompt_tokens", "completion_tokens",
 "total_tokens"}}; ``POST /v1/chat/completions`` with {"messages": [{"role", "content"}], "max_tokens",
 "temperature", "seed", "template"} -> {"object": "chat.completion", "choices": [{"message": {"role":
 "assistant", "content"}, "finish_reason"}], "usage"}: the conversation is rendered with the chat
@@ -359,7 +360,7 @@ class CompletionServer:
     def _answers(self, req: dict) -> Tuple[int, Optional[LogitOptions]]:
         """(number of answers, what changes the logits) of a request."""
         n = req.get("n")
-        n = 1 if n is None else n
+        n = 1 if n is None else int(n) if isinstance(n, float) and n.is_integer() else n
         if isinstance(n, bool) or not isinstance(n, int) or not 1 <= n <= self.max_n:
             raise ValueError(f"n must be a whole number in [1, {self.max_n}]")
         return n, LogitOptions.from_request(req, self.cfg.vocab_size)

@@ -65,3 +65,11 @@ def test_options_made_in_python_are_checked_too():
     for kw in (dict(presence=1e39), dict(frequency=float("inf")), dict(repetition=0.0), dict(bias={3: float("nan")})):
         with pytest.raises(ValueError):
             LogitOptions(**kw)
+
+
+def test_n_of_a_client_that_writes_floats(srv):
+    st, out = _post(srv, {"n": 2.0})
+    assert st == 200 and [c["index"] for c in out["choices"]] == [0, 1]
+    assert len(_post(srv, {"n": 1.0}, "/v1/chat/completions")[1]["choices"]) == 1
+    for bad in (1.5, 0.0, 4.0, float("inf"), float("nan")):
+        assert _post(srv, {"n": bad})[0] == 400
