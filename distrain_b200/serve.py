@@ -181,8 +181,9 @@ def sample_cached(dec, ids: List[int], n: int, max_tokens: int, temperature: flo
                   options: Optional[LogitOptions] = None) -> List[Tuple[List[int], str]]:
     """n answers of up to ``max_tokens`` tokens to one prompt through a ``PagedDecoder``: (new tokens, finish
     reason) of each, drawn like ``sample`` with seeds ``seed``, ``seed + 1``, .... A prompt that leaves too little
-    room loses tokens on the left. Raises if the GPU reports that a step could not be done."""
-    ids = (list(ids) if ids else [1])[-dec.max_prompt:]
+    room loses tokens on the left; penalties see all of it, as in ``sample``. Raises if the GPU reports that a step
+    could not be done."""
+    ids = list(ids) if ids else [1]
     if max_tokens <= 0:
         return [([], "length") for _ in range(n)]
     V, dev = dec.eng.V, dec.dev
@@ -199,7 +200,7 @@ def sample_cached(dec, ids: List[int], n: int, max_tokens: int, temperature: flo
         lens = prompt.clone()
         args = options.device_args(n, history, lens, prompt, V)
     try:
-        logits = dec.prefill(ids).expand(n, V)  # every answer's first token comes from the prompt's last position
+        logits = dec.prefill(ids[-dec.max_prompt:]).expand(n, V)  # every answer's first token comes from the prompt's last position
         for k in range(int(max_tokens)):
             if k:
                 if k == 1:

@@ -96,3 +96,55 @@ def test_answers_whose_buffers_fail_cannot_be_stepped():
         dec.branch(1)
     with pytest.raises(ValueError, match="tokens"):
         dec.step([1])
+
+
+def _plain_process(logits, out, *, history, lens, prompt_lens, repetition, presence, frequency, bias_ids=None,
+                   bias_vals=None, bias_lens=None, mask=None):
+    """The processor's formula, one row after another on the CPU."""
+    for b in range(logits.shape[0]):
+        z = logits[b].clone()
+        h = history[b, :int(lens[b])].long()
+        seen = torch.bincount(h, minlength=z.numel()) > 0
+        count = torch.bincount(h[int(prompt_lens[b]):], minlength=z.numel())
+        z = torch.where(seen, torch.where(z > 0, z / repetition[b], z * repetition[b]), z)
+        z = z - frequency[b] * count - presence[b] * (count > 0)
+        if bias_ids is not None:
+            for e in range(int(bias_lens[b])):
+                z[int(bias_ids[b, e])] += bias_vals[b, e]
+        if mask is not None:
+            v = torch.arange(z.numel())
+            z[(mask[b].long()[v // 32] >> (v % 32)) & 1 == 0] = float("-inf")
+        out[b] = z
+
+
+class _FakeLM:
+    """The fake decoder's logits for ``sample``."""
+
+    def __init__(self, dec):
+        self.dec = dec
+
+    def next_logits(self, seq):
+        return self.dec.z[seq[-1]]
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("options", [None, dict(presence=0.7, frequency=0.3, repetition=1.8, bias={3: 1.5, 40: -2.0}),
+                                     dict(repetition=2.5, allowed=list(range(0, 50, 3)))])
+@pytest.mark.parametrize("prompt", [5, 40])  # 40: longer than the decoder has room for
+def test_answers_follow_sample(monkeypatch, temperature, options, prompt):
+    """Answer i is what ``sample`` draws with seed + i, penalties on the whole prompt among the rest."""
+    from distrain_b200.ops import sampling
+    from distrain_b200.serve import LogitOptions, sample, sample_cached
+    monkeypatch.setattr(sampling, "process_logits", _plain_process)
+    dec = FakeDecoder(seed=4)
+    ids = torch.randint(0, 50, (prompt,), generator=torch.Generator().manual_seed(1)).tolist()
+    o = None if options is None else LogitOptions(**options)
+    got = sample_cached(dec, ids, 4, 12, temperature, 7, options=o)
+    sd = {"x": torch.zeros(1)}
+    want = [sample(sd, None, ids, 12, temperature, 7 + i, lm=_FakeLM(dec), options=o) for i in range(4)]
+    assert got == want
+    if temperature:
+        assert len({tuple(a) for a, _ in got}) > 1
+    stop = got[0][0][3]
+    got = sample_cached(dec, ids, 4, 12, temperature, 7, stop_token=stop, options=o)
+    assert got == [sample(sd, None, ids, 12, temperature, 7 + i, stop_token=stop, lm=_FakeLM(dec), options=o) for i in range(4)]
