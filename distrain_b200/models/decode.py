@@ -12,6 +12,8 @@ same logits from the new tokens alone.
 """
 from __future__ import annotations
 
+import contextlib
+import functools
 from typing import List, Sequence
 
 import torch
@@ -25,6 +27,20 @@ ROWS = 128  # rows of an activation buffer: whole GEMM tiles
 
 def _pad(n: int, a: int) -> int:
     return (n + a - 1) // a * a
+
+
+def on_device(dev: torch.device):
+    """``dev`` as the current device, where kernels are launched. (Which device is current belongs to the calling
+    thread, and a server's handlers have threads of their own.)"""
+    return torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext()
+
+
+def _on_its_device(method):
+    @functools.wraps(method)
+    def run(self, *args, **kw):
+        with on_device(self.dev):
+            return method(self, *args, **kw)
+    return run
 
 
 class PagedDecoder:
@@ -41,6 +57,7 @@ class PagedDecoder:
         pages = self.prompt_pages + self.max_batch * self.answer_pages
         shape = (eng.cfg.num_layers, pages, eng.nkv, self.P, eng.d)
         self.k, self.v = (torch.zeros(shape, dtype=torch.bfloat16, device=self.dev) for _ in range(2))
+        self.dev = self.k.device  # (with its index)
         self.free = torch.arange(pages, dtype=torch.int32, device=self.dev)
         cos, sin = rope_tables(eng.cfg, self.max_prompt + self.max_new)
         self.cos, self.sin = cos.to(self.dev).contiguous(), sin.to(self.dev).contiguous()
@@ -114,6 +131,7 @@ class PagedDecoder:
             if not 0 <= t < self.eng.V:
                 raise ValueError(f"token id {t} outside the vocabulary of {self.eng.V}")
 
+    @_on_its_device
     def prefill(self, ids: Sequence[int]) -> torch.Tensor:
         """Forward of a prompt into fresh pages; fp32 logits [1, V] of the token after it."""
         T = len(ids)
@@ -135,6 +153,7 @@ class PagedDecoder:
         self.prompt_len = T
         return self._logits(hidden[T - 1:T])
 
+    @_on_its_device
     def branch(self, n: int):
         """n answers that continue the prompt; their tokens come with ``step``."""
         if not self.prompt_len:
@@ -154,6 +173,7 @@ class PagedDecoder:
         self.plan = paged.AttentionPlan(self.rows, n, 1, nh=e.nh, nkv=e.nkv, d=e.d, page_size=self.P, device=self.dev)
         self.n = n
 
+    @_on_its_device
     def check(self):
         """Raises if the GPU could not do what the steps since ``prefill`` asked for; their logits are worth nothing then.
         Waits for the GPU: once at the end of an answer is enough. The library's error state is clear afterwards."""
@@ -165,6 +185,7 @@ class PagedDecoder:
         if refused:
             raise RuntimeError(f"generation failed on the GPU: page tables refused a step ({refused})")
 
+    @_on_its_device
     def step(self, tokens: List[int]) -> torch.Tensor:
         """Adds ``tokens[i]`` to answer i; fp32 logits [n, V] of the tokens after them."""
         if len(tokens) != self.n or self.n == 0:

@@ -183,6 +183,7 @@ def sample_cached(dec, ids: List[int], n: int, max_tokens: int, temperature: flo
     reason) of each, drawn like ``sample`` with seeds ``seed``, ``seed + 1``, .... A prompt that leaves too little
     room loses tokens on the left; penalties see all of it, as in ``sample``. Raises if the GPU reports that a step
     could not be done."""
+    from .models.decode import on_device
     ids = list(ids) if ids else [1]
     if max_tokens <= 0:
         return [([], "length") for _ in range(n)]
@@ -208,7 +209,8 @@ def sample_cached(dec, ids: List[int], n: int, max_tokens: int, temperature: flo
                 logits = dec.step([o[-1] for o in out])
             if args is not None:
                 z = torch.empty(n, V, dtype=torch.float32, device=dev)
-                process_logits(logits, z, **args)
+                with on_device(dev):
+                    process_logits(logits, z, **args)
             else:
                 z = logits
             if temperature <= 0:
@@ -278,14 +280,15 @@ def load_decoder(sd, cfg, device: str, max_prompt: int, max_new: int, max_batch:
     """A ``PagedDecoder`` on the weights ``sd`` (a GPU)."""
     if torch.device(device).type != "cuda":
         raise ValueError("the key/value cache needs a CUDA device")
-    from .models.decode import PagedDecoder
+    from .models.decode import PagedDecoder, on_device
     from .models.engine import TrainEngine
     from .models.params import ParamLayout
     L = ParamLayout(cfg)
     flat = torch.zeros(L.total)
     L.load_state_dict(flat, {k: v.detach().float().cpu() for k, v in sd.items()})
-    eng = TrainEngine(cfg, 1, 2, device=device, flat_init=flat, inference=True)  # (weights; its buffers stay unused)
-    return PagedDecoder(eng, max_prompt, max_new, max_batch)
+    with on_device(torch.device(device)):
+        eng = TrainEngine(cfg, 1, 2, device=device, flat_init=flat, inference=True)  # (weights; its buffers stay unused)
+        return PagedDecoder(eng, max_prompt, max_new, max_batch)
 
 
 class CompletionServer:

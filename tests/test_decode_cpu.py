@@ -148,3 +148,58 @@ def test_answers_follow_sample(monkeypatch, temperature, options, prompt):
     stop = got[0][0][3]
     got = sample_cached(dec, ids, 4, 12, temperature, 7, stop_token=stop, options=o)
     assert got == [sample(sd, None, ids, 12, temperature, 7 + i, stop_token=stop, lm=_FakeLM(dec), options=o) for i in range(4)]
+
+
+def test_every_call_runs_on_the_decoders_device(monkeypatch):
+    """The current device is a thread's own: a decoder on another one makes it current around all it launches."""
+    from distrain_b200 import ops, serve
+    from distrain_b200.models import decode, engine
+    from distrain_b200.ops import sampling
+    current, seen = [0], []
+
+    class Device:  # stands in for torch.cuda.device
+        def __init__(self, dev):
+            self.index = torch.device(dev).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+    monkeypatch.setattr(torch.cuda, "device", Device)
+
+    def note(*a, **kw):
+        seen.append(current[0])
+        raise KeyError("seen")
+    dec = _decoder(dev=torch.device("cuda", 1), prompt_len=3, rows=128, eng=SimpleNamespace(V=100, H=8))
+    dec._buffers = dec._ints = note
+    monkeypatch.setattr(ops, "device_error", note)
+    for call in (lambda: dec.step([1, 2]), lambda: dec.prefill([1]), dec.check):
+        with pytest.raises(KeyError):
+            call()
+    monkeypatch.setattr(torch, "full", note)
+    with pytest.raises(KeyError):
+        dec.prompt_len = 3
+        dec.prompt_pages = dec.answer_pages = 1
+        dec.P = 16
+        dec.branch(1)
+    monkeypatch.undo()
+    assert seen == [1] * 4 and current == [0]
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(engine, "TrainEngine", note)
+    from distrain_b200.config import ModelConfig
+    cfg = ModelConfig(hidden_dim=32, num_layers=1, num_heads=4, num_kv_heads=2, ffn_hidden_dim=64, vocab_size=64, max_seq_len=32)
+    from distrain_b200.models.params import ParamLayout, init_flat
+    L = ParamLayout(cfg)
+    with pytest.raises(KeyError):
+        serve.load_decoder(L.to_state_dict(init_flat(L, seed=1)), cfg, "cuda:1", 8, 8)
+    fake = FakeDecoder()
+
+    def processor(logits, out, **kw):
+        seen.append(current[0])
+        out.copy_(logits)
+    monkeypatch.setattr(sampling, "process_logits", processor)
+    monkeypatch.setattr(decode, "on_device", lambda dev: Device("cuda:2"))
+    serve.sample_cached(fake, [1], 1, 2, options=serve.LogitOptions(presence=1.0))
+    assert seen[4:] == [1, 2, 2] and current == [0]
