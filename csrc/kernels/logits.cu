@@ -14,6 +14,7 @@
 // (26 MB, 4.3 TB/s); 20 us for 256 rows of 32768 bf16 logits with histories of 4096, biases and masks (54 MB, 2.7
 // TB/s): there 71% of the issue slots are taken, by the history and by the counter of every logit.
 #include "common.cuh"
+#include "spans.h"
 
 // Arguments of the launcher (pointers and 64-bit values first, then ints, no padding). Null pointers leave their part
 // out; `lens` goes with `history`, `bias_lens` with the bias lists.
@@ -186,6 +187,17 @@ DT_API int dt_process_logits(const LogitsArgs* args, cudaStream_t st) {
       a.max_history > COUNT)
     return -10;
   if (a.B == 0) return 0;
+  const long long B = a.B, V = a.V, e = a.bf16 ? 2 : 4;
+  const bool in_place = a.x == a.out && !a.bf16 && a.ldx == a.ldo;  // each element is read by the thread that writes it
+  const Span out[] = {span_rows(a.out, B, 4 * V, 4 * a.ldo)};
+  const Span in[] = {span_rows(in_place ? nullptr : a.x, B, e * V, e * a.ldx),
+                     span_rows(a.history, B, 4LL * a.max_history, 4 * a.ldh),
+                     span(a.prompt_lens, 4 * B), span(a.lens, 4 * B),
+                     span(a.repetition, 4 * B), span(a.presence, 4 * B), span(a.frequency, 4 * B),
+                     span_rows(a.bias_ids, B, 4LL * a.max_bias, 4 * a.ldb),
+                     span_rows(a.bias_vals, B, 4LL * a.max_bias, 4 * a.ldb), span(a.bias_lens, 4 * B),
+                     span_rows(a.mask, B, (V + 31) / 32 * 4, 4 * a.ldm)};
+  if (outputs_shared(out, in)) return -13;
   // Four elements at a time where row and column offsets keep input and output on the same phase of four: both
   // strides agree modulo 4 and both bases sit on the same element of a group.
   const uintptr_t xb = reinterpret_cast<uintptr_t>(a.x), ob = reinterpret_cast<uintptr_t>(a.out);

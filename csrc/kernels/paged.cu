@@ -4,6 +4,7 @@
 // (the unit the attention kernel fetches). A token's slot is page * page_size + offset; slots are 32-bit
 // (the host refuses caches of 2^31 tokens or more), every element offset is 64-bit.
 #include "common.cuh"
+#include "spans.h"
 #include <atomic>
 
 namespace {
@@ -265,6 +266,11 @@ DT_API int dt_page_tables(const PageTablesArgs* args, cudaStream_t st) {
   const PageTablesArgs& a = *args;
   if (a.B < 1 || a.B > PT_MAX_REQUESTS || a.cap < 0 || a.n_free < 0 || a.width < 0 || a.shift < 0 || a.shift > 16)
     return -10;
+  const long long B = a.B, cap = a.cap;
+  const Span out[] = {span_rows(a.tables, B, 4LL * a.width, 4 * a.ld), span(a.slots, 4 * cap), span(a.positions, 4 * cap),
+                      span(a.cu, 4 * (B + 1)), span(a.total, 4 * B), span(a.used, 8)};
+  const Span in[] = {span(a.cached, 4 * B), span(a.fresh, 4 * B), span(a.start, 4 * B), span(a.free_pages, 4LL * a.n_free)};
+  if (outputs_shared(out, in)) return -13;
   const int smem = 3 * a.B * (int)sizeof(int);
   const int rc = page_tables_prepared(smem);
   if (rc) return rc;
@@ -275,6 +281,12 @@ DT_API int dt_page_tables(const PageTablesArgs* args, cudaStream_t st) {
                                                      a.width, a.slots, a.positions, a.cap, a.cu, a.total, a.used, a.B,
                                                      a.shift);
   return (int)cudaGetLastError();
+}
+
+// Whether two sets of rows share memory (spans.h): 0 or 1.
+DT_API int dt_spans_meet(const void* p, long long rows, long long bytes, long long stride, const void* p2, long long rows2,
+                         long long bytes2, long long stride2) {
+  return spans_meet(span_rows(p, rows, bytes, stride), span_rows(p2, rows2, bytes2, stride2));
 }
 
 struct KvAppendArgs {
@@ -295,6 +307,11 @@ DT_API int dt_kv_append(const KvAppendArgs* args, cudaStream_t st) {
        reinterpret_cast<uintptr_t>(a.sinT)) & 15)
     return -11;
   if (T == 0) return 0;
+  const long long cache = 2LL * a.num_pages * nkv * d << a.shift, W = (long long)(nh + 2 * nkv) * d;
+  const Span out[] = {span(a.q, 2LL * T * nh * d), span(a.kc, cache), span(a.vc, cache)};
+  const Span in[] = {span_rows(a.qkv, T, 2 * W, 2 * a.ld), span(a.bias, 4 * W), span(a.cosT, 2LL * a.max_pos * d),
+                     span(a.sinT, 2LL * a.max_pos * d), span(a.slots, 4LL * T), span(a.positions, 4LL * T)};
+  if (outputs_shared(out, in)) return -13;
   const int items = (nh + nkv) * (d / 16) + nkv * d / 8;
   const int threads = items >= 256 ? 256 : (items + 31) / 32 * 32;
   const bool wide = T >= 2048;  // enough tokens that half of the blocks still fills the GPU

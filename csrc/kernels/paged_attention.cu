@@ -16,6 +16,7 @@
 // serves every layer of the step. An item costs its key tiles plus a few units for its start and end (loading its
 // queries, filling the pipeline, writing its rows), so that a CTA with many short items gets fewer tiles.
 #include "common.cuh"
+#include "spans.h"
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <atomic>
@@ -1668,6 +1669,12 @@ int shape_of(Shape* s, int T, int B, int G, int nh, int nkv, int d) {
   return 0;
 }
 
+long long plan_bytes(const Shape& s) {
+  return (long long)(H_INTS + (s.G + s.B + 7) / 8 * 8 + (s.B + 7) / 8 * 8) * 4 +
+         ((long long)s.max_entries[STREAM] + s.max_entries[WIDE]) * (long long)sizeof(Entry);
+}
+long long work_bytes(const Shape& s) { return s.part_rows * (s.d + 1) * 4; }
+
 // launch that may begin while the kernel before it in the stream still runs (see pdl_wait)
 template <typename... P, typename... A>
 cudaError_t launch_early(void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t st, const A&... args) {
@@ -1732,14 +1739,13 @@ DT_API long long dt_paged_plan_bytes(int T, int B, int G, int nh, int nkv, int d
   Shape s;
   const int rc = shape_of(&s, T, B, G, nh, nkv, d);
   if (rc) return rc < 0 ? rc : -1;
-  return (long long)(H_INTS + (G + B + 7) / 8 * 8 + (B + 7) / 8 * 8) * 4 +
-         ((long long)s.max_entries[STREAM] + s.max_entries[WIDE]) * (long long)sizeof(Entry);
+  return plan_bytes(s);
 }
 DT_API long long dt_paged_work_bytes(int T, int B, int G, int nh, int nkv, int d) {
   Shape s;
   const int rc = shape_of(&s, T, B, G, nh, nkv, d);
   if (rc) return rc < 0 ? rc : -1;
-  return s.part_rows * (d + 1) * 4;
+  return work_bytes(s);
 }
 // Kernels that dt_paged_attention launches for a shape.
 DT_API int dt_paged_kernels(int T, int B, int G, int nh, int nkv, int d) {
@@ -1782,7 +1788,7 @@ struct PagedAttentionArgs {
   const int *cu_q, *cu_group, *tables, *prefix_tables;
   long long ld_tables, ld_prefix;
   double scale;
-  int T, B, G, nh, nkv, d, shift, pages;
+  int T, B, G, nh, nkv, d, shift, pages, width, prefix_width;
 };
 DT_API int dt_paged_attention(const PagedAttentionArgs* args, cudaStream_t st) {
   const PagedAttentionArgs& g = *args;
@@ -1794,6 +1800,13 @@ DT_API int dt_paged_attention(const PagedAttentionArgs* args, cudaStream_t st) {
        reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.work) | reinterpret_cast<uintptr_t>(g.plan)) & 15)
     return -11;
   if (g.T == 0) return 0;
+  const long long rows = (long long)g.T * g.nh, cache = 2LL * g.pages * g.nkv * g.d << g.shift;
+  const Span out[] = {span(g.out, 2 * rows * g.d), span(g.lse, 4 * rows), span(g.work, work_bytes(s))};
+  const Span in[] = {span(g.q, 2 * rows * g.d), span(g.kc, cache), span(g.vc, cache), span(g.plan, plan_bytes(s)),
+                     span(g.cu_q, 4LL * (g.B + 1)), span(g.cu_group, 4LL * (g.G + 1)),
+                     span_rows(g.tables, g.B, 4LL * g.width, 4 * g.ld_tables),
+                     span_rows(g.prefix_tables, g.G, 4LL * g.prefix_width, 4 * g.ld_prefix)};
+  if (outputs_shared(out, in)) return -13;
   float* po = reinterpret_cast<float*>(g.work);
   const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(g.q), reinterpret_cast<__nv_bfloat16*>(g.out), g.lse, g.plan,
                    g.tables, g.prefix_tables, g.ld_tables, g.ld_prefix, g.cu_q, g.cu_group, po, po + s.part_rows * g.d,

@@ -38,7 +38,7 @@ _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 _TABLES = struct.Struct("=10Qq6i").pack
 _APPEND = struct.Struct("=9Qq8i").pack
 _PLAN = struct.Struct("=5Q10i").pack
-_ATTENTION = struct.Struct("=11Q2qd8i").pack
+_ATTENTION = struct.Struct("=11Q2qd10i").pack
 
 _fns = {}
 
@@ -60,6 +60,14 @@ def _fn(name):
 
 def _fail(msg):
     raise ValueError(msg)
+
+
+def _launch(name, args, stream):
+    """Calls a launcher, which sees for itself what depends on addresses."""
+    rc = _fn(name)(args, stream)
+    if rc == -13:
+        _fail(f"{name[3:]}: outputs must not share memory with inputs or each other")
+    check(rc, name)
 
 
 def _vec(name, t, n, dtype=_I32):
@@ -158,8 +166,8 @@ def page_tables(cached, new, free, tables, slots, positions, cu, total, used, *,
             total.get_device() == dev and used.get_device() == dev and (start is None or start.get_device() == dev) and
             _current() == dev):
         on_current_device(cached, new, free, tables, slots, positions, cu, total, used, start)
-    check(_fn("dt_page_tables")(_TABLES(a, b, s, f, *o, tables.stride(0), n_free, ts[1], n[0], B, shift, 0),
-                                _stream(stream, dev)), "dt_page_tables")
+    _launch("dt_page_tables", _TABLES(a, b, s, f, *o, tables.stride(0), n_free, ts[1], n[0], B, shift, 0),
+            _stream(stream, dev))
 
 
 def _cache(k_cache, v_cache):
@@ -183,7 +191,8 @@ def kv_append(qkv, bias, cos, sin, slots, positions, q, k_cache, v_cache, *, str
     ``qkv`` [T, (nh + 2 nkv) d] bf16 (rows may be strided: the QKV GEMM's output without bias), ``bias`` fp32
     or None, ``cos`` / ``sin`` [max_pos, d/2] fp32 tables of the rotate-half form. Row t with slot ``slots[t]``
     >= 0: ``q[t]`` = rot(q + bias), K row = rot(k + bias), V row = v + bias, each rounded once to bf16; a row
-    with a negative slot is left out (its ``q`` row too). Two rows of one call must not have the same slot.
+    with a negative slot is left out (its ``q`` row too). Two rows of one call must not have the same slot, and
+    ``q``, ``k_cache`` and ``v_cache`` must not share memory with each other or an input.
     A slot outside the cache or a position outside the tables leaves its row out and is reported."""
     pages, nkv, page_size, d = _cache(k_cache, v_cache)
     rows, qs, cs = qkv.shape, q.shape, cos.shape
@@ -220,10 +229,10 @@ def kv_append(qkv, bias, cos, sin, slots, positions, q, k_cache, v_cache, *, str
         on_current_device(qkv, bias, cos, sin, slots, positions, q, k_cache, v_cache)
     if T == 0:
         return
-    check(_fn("dt_kv_append")(_APPEND(qkv.data_ptr(), 0 if bias is None else bias.data_ptr(), cos.data_ptr(),
-                                      sin.data_ptr(), slots.data_ptr(), positions.data_ptr(), q.data_ptr(),
-                                      k_cache.data_ptr(), v_cache.data_ptr(), ld, cs[0], T, nh, nkv, d,
-                                      _SHIFT[page_size], pages, 0), _stream(stream, dev)), "dt_kv_append")
+    _launch("dt_kv_append", _APPEND(qkv.data_ptr(), 0 if bias is None else bias.data_ptr(), cos.data_ptr(),
+                                    sin.data_ptr(), slots.data_ptr(), positions.data_ptr(), q.data_ptr(),
+                                    k_cache.data_ptr(), v_cache.data_ptr(), ld, cs[0], T, nh, nkv, d,
+                                    _SHIFT[page_size], pages, 0), _stream(stream, dev))
 
 
 class AttentionPlan:
@@ -306,7 +315,8 @@ def paged_attention(q, k_cache, v_cache, out, plan, *, scale=None, lse=None, str
     0 .. lens - n + j. ``q`` and ``out`` [T, nh * d] bf16, T = the plan's tokens; rows behind ``cu_q[B]`` are
     left as they are. ``scale`` defaults to d ** -0.5. ``lse`` [T, nh] fp32 receives the log-sum-exp of the
     scaled scores. A token that sees no key gets a zero row (lse -inf). What the pages hold behind a request's
-    last key does not matter; a non-finite V row of a *later* token of the same request may reach earlier ones."""
+    last key does not matter; a non-finite V row of a *later* token of the same request may reach earlier ones. ``out``
+    and ``lse`` must not share memory with each other or an input."""
     pages, nkv, page_size, d = _cache(k_cache, v_cache)
     if nkv != plan.nkv or page_size != plan.page_size or d != plan.d:
         _fail(f"cache of {nkv} kv heads, pages of {page_size}, head dim {d}; plan for {plan.nkv}, {plan.page_size}, {plan.d}")
@@ -333,10 +343,11 @@ def paged_attention(q, k_cache, v_cache, out, plan, *, scale=None, lse=None, str
         on_current_device(q, k_cache, v_cache, out, lse, plan.plan)
     if T == 0:
         return
-    pt, ld_prefix, cg = (0, 0, 0) if prefix is None else (prefix[0].data_ptr(), prefix[0].stride(0), prefix[2].data_ptr())
-    check(_fn("dt_paged_attention")(_ATTENTION(qp, k_cache.data_ptr(), v_cache.data_ptr(), op,
-                                               0 if lse is None else lse.data_ptr(), plan.plan.data_ptr(),
-                                               plan.work.data_ptr(), cu_q.data_ptr(), cg, tables.data_ptr(), pt,
-                                               tables.stride(0), ld_prefix, scale, T, plan.B, plan.G, nh, nkv, d,
-                                               plan.shift, pages), _stream(stream, dev)), "dt_paged_attention")
+    pt, ld_prefix, cg, wp = (0, 0, 0, 0) if prefix is None else \
+        (prefix[0].data_ptr(), prefix[0].stride(0), prefix[2].data_ptr(), prefix[0].shape[1])
+    _launch("dt_paged_attention", _ATTENTION(qp, k_cache.data_ptr(), v_cache.data_ptr(), op,
+                                             0 if lse is None else lse.data_ptr(), plan.plan.data_ptr(),
+                                             plan.work.data_ptr(), cu_q.data_ptr(), cg, tables.data_ptr(), pt,
+                                             tables.stride(0), ld_prefix, scale, T, plan.B, plan.G, nh, nkv, d,
+                                             plan.shift, pages, tables.shape[1], wp), _stream(stream, dev))
     LAUNCHES[0] += plan.kernels - 1

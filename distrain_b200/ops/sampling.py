@@ -5,8 +5,7 @@ import struct
 
 import torch
 
-from ._lib import check
-from .paged import _F32, _I32, _fail, _fn, _stream, _vec, on_current_device
+from .paged import _F32, _I32, _fail, _launch, _stream, _vec, on_current_device
 
 MAX_BIAS = 16384
 _LOGITS = struct.Struct("=12Q5q6i").pack  # argument struct of the launcher (csrc/kernels/logits.cu)
@@ -21,7 +20,8 @@ def _matrix(name, t, rows, cols, dtype):
 
 def process_logits(logits, out, *, history=None, lens=None, prompt_lens=None, repetition=None, presence=None,
                    frequency=None, bias_ids=None, bias_vals=None, bias_lens=None, mask=None, stream=None):
-    """``out`` [B, V] fp32 from ``logits`` [B, V] (fp32 or bf16; rows may be strided; fp32 ``out`` may be ``logits``).
+    """``out`` [B, V] fp32 from ``logits`` [B, V] (fp32 or bf16; rows may be strided; fp32 ``out`` may be ``logits``,
+    and shares memory with no input otherwise).
 
     With c = how often token v occurs in ``history[b, prompt_lens[b]:lens[b]]`` (the answer so far; the whole
     row without ``prompt_lens``) and *seen* = it occurs in ``history[b, :lens[b]]``, in this order:
@@ -96,6 +96,5 @@ def process_logits(logits, out, *, history=None, lens=None, prompt_lens=None, re
                             bias_lens, mask)
     if B == 0:
         return
-    check(_fn("dt_process_logits")(_LOGITS(xp, op, hp, np, pp, rp, ap, fp, ip, vp, cp, mp, ldx, ldo, ldh, ldb, ldm,
-                                           logits.dtype is torch.bfloat16, B, V, L, K, 0), _stream(stream, dev)),
-          "dt_process_logits")
+    _launch("dt_process_logits", _LOGITS(xp, op, hp, np, pp, rp, ap, fp, ip, vp, cp, mp, ldx, ldo, ldh, ldb, ldm,
+                                         logits.dtype is torch.bfloat16, B, V, L, K, 0), _stream(stream, dev))

@@ -73,3 +73,28 @@ def test_n_of_a_client_that_writes_floats(srv):
     assert len(_post(srv, {"n": 1.0}, "/v1/chat/completions")[1]["choices"]) == 1
     for bad in (1.5, 0.0, 4.0, float("inf"), float("nan")):
         assert _post(srv, {"n": bad})[0] == 400
+
+
+# ───────────────────────── buffers that share memory ─────────────────────────
+def test_spans_meet_where_a_byte_is_in_both():
+    """The launchers' test of buffers against the sets of their bytes; nothing is read there."""
+    import ctypes
+    import random
+    from distrain_b200.ops._lib import lib
+    f = lib().dt_spans_meet
+    f.argtypes, f.restype = [ctypes.c_void_p] + [ctypes.c_longlong] * 3 + [ctypes.c_void_p] + [ctypes.c_longlong] * 3, ctypes.c_int
+    rng, base, hits = random.Random(0), 1 << 40, 0
+    for _ in range(20000):
+        spans, sets = [], []
+        for _ in range(2):
+            at, rows, nbytes = rng.randint(0, 60), rng.randint(1, 6), rng.randint(1, 12)
+            stride = rng.choice([0, nbytes, nbytes + rng.randint(0, 20), rng.randint(1, 12)])
+            spans += [base + at, rows, nbytes, stride]
+            sets.append({at + r * stride + i for r in range(rows) for i in range(nbytes)})
+        want = bool(sets[0] & sets[1])
+        hits += want
+        assert f(*spans) == want, spans
+    assert 4000 < hits < 16000
+    assert f(base, 0, 4, 4, base, 1, 4, 4) == 0 and f(base, 1, 0, 0, base, 1, 4, 4) == 0 and f(0, 1, 8, 8, 0, 1, 8, 8) == 0
+    far = 1 << 33  # spans past 32 bits
+    assert f(base, 2, 4, far, base + far, 1, 4, 4) == 1 and f(base, 2, 4, far, base + far + 4, 1, 4, 4) == 0

@@ -152,3 +152,96 @@ def test_generation_fails_on_what_the_gpu_reports():
         dec.branch = branch
         assert ops.device_error() == (0, 0)
         assert sample_cached(dec, ids, 2, 20) == want
+
+
+# ───────────────────────── buffers that share memory ─────────────────────────
+def _zeros(*s, dtype=torch.bfloat16):
+    return torch.zeros(*s, dtype=dtype, device=DEV)
+
+
+def test_shifted_views_of_one_buffer_are_refused():
+    """An output that begins at another element than an input, but lies over it."""
+    from distrain_b200.ops import paged, sampling
+    i32, f32 = torch.int32, torch.float32
+    refused = lambda: pytest.raises(ValueError, match="share memory")  # noqa: E731
+    # page tables: every output against an input and another output
+    names = ["tables", "slots", "positions", "cu", "total", "used"]
+    def tables(**kw):
+        a = dict(cached=_zeros(8, dtype=i32), new=_zeros(8, dtype=i32), free=_zeros(9, dtype=i32), tables=_zeros(8, 4, dtype=i32),
+                 slots=_zeros(8, dtype=i32), positions=_zeros(8, dtype=i32), cu=_zeros(9, dtype=i32),
+                 total=_zeros(8, dtype=i32), used=_zeros(2, dtype=i32), start=_zeros(8, dtype=i32))
+        for name, t in kw.items():
+            assert t.shape == a[name].shape
+        a.update(kw)
+        paged.page_tables(**a, page_size=16)
+    tables()
+    sizes = dict(tables=32, slots=8, positions=8, cu=9, total=8, used=2, cached=8, new=8, free=9, start=8)
+    for out in names:
+        for other in ["cached", "new", "free", "start"] + [n for n in names if n != out]:
+            buf = _zeros(64, dtype=i32)
+            x, y = buf[:sizes[out]], buf[1:1 + sizes[other]]
+            shape = lambda n, t: t.view(8, 4) if n == "tables" else t  # noqa: E731
+            with refused():
+                tables(**{out: shape(out, x), other: shape(other, y)})
+    wide = _zeros(8, 16, dtype=i32)
+    tables(tables=wide[:, :4], cu=wide[0, 4:13], total=wide[1, 4:12])  # in the gaps of the rows: not shared
+    with refused():
+        tables(tables=wide[:, :4], total=wide.view(-1)[28:36])  # into row 2
+    # append
+    d, P, nh, nkv, T = 32, 16, 4, 2, 4
+    def append(**kw):
+        a = dict(qkv=_zeros(T, 8 * d), bias=_zeros(8 * d, dtype=f32), cos=_zeros(8, 16, dtype=f32), sin=_zeros(8, 16, dtype=f32),
+                 slots=_i([0, 1, 2, 3]), positions=_i([0, 1, 2, 3]), q=_zeros(T, nh * d), k_cache=_zeros(2, nkv, P, d),
+                 v_cache=_zeros(2, nkv, P, d))
+        a.update(kw)
+        paged.kv_append(**a)
+    append()
+    k = _zeros(3, nkv, P, d)
+    buf = _zeros(T * 8 * d + 8)
+    for kw in (dict(k_cache=k[:2], v_cache=k[1:]), dict(k_cache=k[:2], v_cache=k[:2]),
+               dict(qkv=buf[:T * 8 * d].view(T, 8 * d), q=buf[8:8 + T * nh * d].view(T, nh * d)),
+               dict(qkv=k.view(-1)[8:8 + T * 8 * d].view(T, 8 * d), k_cache=k[:2])):
+        with refused():
+            append(**kw)
+    # attention
+    cu, lens, tb = _i([0, 4]), _i([4]), _i([[0]])
+    def attend(groups=0, **kw):
+        plan = paged.AttentionPlan(T, 1, groups, nh=nh, nkv=nkv, d=d, page_size=P)
+        plan.build(cu, lens, tb, prefix=(_i([[1]]), _i([3]), _i([0, 1])) if groups else None)
+        a = dict(q=_zeros(T, nh * d), k_cache=_zeros(2, nkv, P, d), v_cache=_zeros(2, nkv, P, d), out=_zeros(T, nh * d))
+        a.update(kw)
+        paged.paged_attention(plan=plan, **a)
+    attend()
+    attend(groups=1)
+    both = _zeros(T * nh * d + 8)
+    n = T * nh * d
+    with refused():
+        attend(q=both[:n].view(T, -1), out=both[8:8 + n].view(T, -1))
+    with refused():
+        attend(k_cache=k[:2], out=k.view(-1)[8:8 + n].view(T, -1))
+    with refused():
+        attend(q=both[:n].view(T, -1), lse=both.view(f32)[4:4 + T * nh].view(T, nh))
+    with refused():
+        attend(out=both[:n].view(T, -1), lse=both.view(f32)[4:4 + T * nh].view(T, nh))
+    same = _zeros(2, nkv, P, d)
+    attend(k_cache=same, v_cache=same)  # inputs may be one another
+    # logits
+    B, V = 4, 50
+    z = _zeros(B * V + 4, dtype=f32)
+    x, o = z[:B * V].view(B, V), z[4:4 + B * V].view(B, V)
+    with refused():
+        sampling.process_logits(x, o)
+    sampling.process_logits(x, x)  # in place
+    pair = _zeros(B, 2 * V, dtype=f32)
+    pair.normal_()
+    left = pair[:, :V].clone()
+    sampling.process_logits(pair[:, :V], pair[:, V:])  # side by side
+    assert torch.equal(pair[:, V:], left) and torch.equal(pair[:, :V], left)
+    with refused():
+        sampling.process_logits(pair[:, :V], pair[:, V - 1:2 * V - 1])
+    with refused():
+        sampling.process_logits(_zeros(B, V, dtype=f32), x, history=z.view(i32)[:B * 5].view(B, 5), lens=_i([1] * B))
+    with refused():
+        sampling.process_logits(_zeros(B, V, dtype=f32), x, mask=z.view(i32)[2:2 + B * 2].view(B, 2))
+    with refused():
+        sampling.process_logits(_zeros(B, V), x, history=_zeros(B, 5, dtype=i32), lens=_i([1] * B), presence=z[8:8 + B])
