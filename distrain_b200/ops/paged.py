@@ -67,6 +67,8 @@ def _launch(name, args, stream):
     rc = _fn(name)(args, stream)
     if rc == -13:
         _fail(f"{name[3:]}: outputs must not share memory with inputs or each other")
+    if rc == -11:
+        _fail(f"{name[3:]}: rows and tables of floats must start on a 16-byte boundary")
     check(rc, name)
 
 

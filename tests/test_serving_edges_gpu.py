@@ -245,3 +245,33 @@ def test_shifted_views_of_one_buffer_are_refused():
         sampling.process_logits(_zeros(B, V, dtype=f32), x, mask=z.view(i32)[2:2 + B * 2].view(B, 2))
     with refused():
         sampling.process_logits(_zeros(B, V), x, history=_zeros(B, 5, dtype=i32), lens=_i([1] * B), presence=z[8:8 + B])
+
+
+def test_rows_off_a_16_byte_boundary_are_refused():
+    """Like every other argument that does not fit: a ValueError, and nothing written."""
+    from distrain_b200.ops import paged
+    d, P, nh, nkv, T = 32, 16, 4, 2, 4
+    def view(*shape, dtype=torch.bfloat16, off=4):
+        n = 1
+        for s in shape:
+            n *= s
+        return torch.ones(n + 16, dtype=dtype, device=DEV)[off:off + n].view(*shape)
+    off = dict(qkv=view(T, 8 * d), bias=view(8 * d, dtype=torch.float32, off=1), cos=view(8, 16, dtype=torch.float32, off=2),
+               sin=view(8, 16, dtype=torch.float32, off=3), q=view(T, nh * d), k_cache=view(2, nkv, P, d),
+               v_cache=view(2, nkv, P, d))
+    for name, t in off.items():
+        a = dict(qkv=_zeros(T, 8 * d), bias=None, cos=_zeros(8, 16, dtype=torch.float32),
+                 sin=_zeros(8, 16, dtype=torch.float32), slots=_i([0, 1, 2, 3]), positions=_i([0, 1, 2, 3]), q=_zeros(T, nh * d),
+                 k_cache=_zeros(2, nkv, P, d), v_cache=_zeros(2, nkv, P, d))
+        a[name] = t
+        with pytest.raises(ValueError, match="16-byte"):
+            paged.kv_append(**a)
+        assert (t == 1).all()
+    plan = paged.AttentionPlan(T, 1, nh=nh, nkv=nkv, d=d, page_size=P)
+    plan.build(_i([0, 4]), _i([4]), _i([[0]]))
+    for name in ("q", "k_cache", "v_cache", "out"):
+        a = dict(q=_zeros(T, nh * d), k_cache=_zeros(2, nkv, P, d), v_cache=_zeros(2, nkv, P, d), out=_zeros(T, nh * d))
+        a[name] = view(*a[name].shape)
+        with pytest.raises(ValueError, match="16-byte"):
+            paged.paged_attention(plan=plan, **a)
+        assert (a[name] == 1).all()
