@@ -315,10 +315,10 @@ def paged_attention(q, k_cache, v_cache, out, plan, *, scale=None, lse=None, str
 
     Token j of a request with n query rows and ``lens`` own keys sees its group's whole prefix and its own keys
     0 .. lens - n + j. ``q`` and ``out`` [T, nh * d] bf16, T = the plan's tokens; rows behind ``cu_q[B]`` are
-    left as they are. ``scale`` defaults to d ** -0.5. ``lse`` [T, nh] fp32 receives the log-sum-exp of the
-    scaled scores. A token that sees no key gets a zero row (lse -inf). What the pages hold behind a request's
-    last key does not matter; a non-finite V row of a *later* token of the same request may reach earlier ones. ``out``
-    and ``lse`` must not share memory with each other or an input."""
+    left as they are. ``scale`` (1e-30 to 1e30; scaled scores stay below 2^30) defaults to d ** -0.5. ``lse`` [T, nh]
+    fp32 receives the log-sum-exp of the scaled scores. A token that sees no key gets a zero row (lse -inf). What the
+    pages hold behind a request's last key does not matter; a non-finite V row of a *later* token of the same request
+    may reach earlier ones. ``out`` and ``lse`` must not share memory with each other or an input."""
     pages, nkv, page_size, d = _cache(k_cache, v_cache)
     if nkv != plan.nkv or page_size != plan.page_size or d != plan.d:
         _fail(f"cache of {nkv} kv heads, pages of {page_size}, head dim {d}; plan for {plan.nkv}, {plan.page_size}, {plan.d}")
@@ -335,8 +335,8 @@ def paged_attention(q, k_cache, v_cache, out, plan, *, scale=None, lse=None, str
     if op == qp and T:
         _fail("out must not be q")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < float("inf"):
-        _fail(f"scale {scale}: a positive number")
+    if not 1e-30 <= scale <= 1e30:  # (zero or infinite in fp32, a masked score's product with it would be NaN)
+        _fail(f"scale {scale}: a number from 1e-30 to 1e30")
     if lse is not None:
         _rows("lse", lse, (T, nh), _F32)
     dev = q.get_device()

@@ -98,3 +98,17 @@ def test_spans_meet_where_a_byte_is_in_both():
     assert f(base, 0, 4, 4, base, 1, 4, 4) == 0 and f(base, 1, 0, 0, base, 1, 4, 4) == 0 and f(0, 1, 8, 8, 0, 1, 8, 8) == 0
     far = 1 << 33  # spans past 32 bits
     assert f(base, 2, 4, far, base + far, 1, 4, 4) == 1 and f(base, 2, 4, far, base + far + 4, 1, 4, 4) == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, 1e-46, 9e-31, 1e39, 1.1e30, float("inf"), float("nan")])
+def test_attention_scales_past_the_edge_of_fp32_are_refused(scale):
+    from distrain_b200.ops import paged
+    from test_paged_cpu import _Plan, _i
+    plan = _Plan(6, 3, 0, 4, 2, 32, 16)
+    plan.cu_q, plan.tables = _i(4), _i(3, 5)
+    b16 = lambda *s: torch.zeros(*s).bfloat16()  # noqa: E731
+    a = (b16(6, 128), b16(3, 2, 16, 32), b16(3, 2, 16, 32), b16(6, 128), plan)
+    with pytest.raises(ValueError, match="scale"):
+        paged.paged_attention(*a, scale=scale)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.paged_attention(*a, scale=1e-30)

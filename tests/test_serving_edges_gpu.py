@@ -275,3 +275,11 @@ def test_rows_off_a_16_byte_boundary_are_refused():
         with pytest.raises(ValueError, match="16-byte"):
             paged.paged_attention(plan=plan, **a)
         assert (a[name] == 1).all()
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-3])
+def test_small_scales(scale):
+    """Weights that are all alike, in both kernels, with rows that see nothing."""
+    from test_paged_gpu import Batch
+    Batch([1, 60, 3], [400, 90, 2], 4, 2, 64, 16).check(scale=scale)
+    Batch([1, 60, 3], [400, 90, 2], 4, 2, 64, 16, pre=[70, 0], sizes=[2, 1]).check(scale=scale)
