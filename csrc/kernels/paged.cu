@@ -75,7 +75,8 @@ page_tables_kernel(const int* __restrict__ cached, const int* __restrict__ fresh
         err = PT_NEGATIVE;
       } else {
         const long long pages = ((long long)c + n + P - 1) >> shift;
-        if (pages > width) err = PT_WIDTH;
+        // (lengths near 2^31, which no table row reaches in int32 slots, would wrap in the 32-bit sums below)
+        if (pages > width || (long long)c + n > 0x7fffffff - P) err = PT_WIDTH;
         v.a = n;
         v.b = pages - (((long long)c + P - 1) >> shift);
       }

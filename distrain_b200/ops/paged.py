@@ -124,8 +124,9 @@ def page_tables(cached, new, free, tables, slots, positions, cu, total, used, *,
     of a shared prefix). ``slots`` may hold more than the step's tokens (a captured graph's capacity): those
     behind get slot -1, which ``kv_append`` skips, those on a page id that is negative or too large for an int32 slot
     get 2^31 - 1, which it reports. ``used`` [2] = pages taken, and why nothing was: 0, or a sum
-    of POOL_EMPTY, TABLE_FULL, SLOTS_FULL, NEGATIVE_LENGTH - then the table is untouched, every slot is -1,
-    ``cu`` is zero and ``total`` equals ``cached``. Outputs must not share memory with inputs."""
+    of POOL_EMPTY, TABLE_FULL (a request of about 2^31 tokens too), SLOTS_FULL, NEGATIVE_LENGTH - then the table is
+    untouched, every slot is -1, ``cu`` is zero and ``total`` equals ``cached``. Outputs must not share memory with
+    inputs or each other."""
     shift = _SHIFT.get(page_size)
     rows, n = cached.shape, slots.shape
     B, ts = rows[0] if len(rows) == 1 else 0, tables.shape

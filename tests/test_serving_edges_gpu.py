@@ -283,3 +283,18 @@ def test_small_scales(scale):
     from test_paged_gpu import Batch
     Batch([1, 60, 3], [400, 90, 2], 4, 2, 64, 16).check(scale=scale)
     Batch([1, 60, 3], [400, 90, 2], 4, 2, 64, 16, pre=[70, 0], sizes=[2, 1]).check(scale=scale)
+
+
+@pytest.mark.parametrize("cached,new", [(2 ** 31 - 10, 5), (2 ** 31 - 1, 0), (2 ** 31 - 17, 2), (0, 2 ** 31 - 1)])
+def test_lengths_near_2_to_31_are_refused(cached, new):
+    """A table row wide enough for them would otherwise be read and written at offsets that have wrapped."""
+    from distrain_b200.ops import paged
+    B, P, width = 2, 16, 2 ** 27 + 8
+    tables = torch.full((B, width), 7, dtype=torch.int32, device=DEV)
+    slots, pos = _i([99] * 8), _i([99] * 8)
+    cu, total, used = _i([99] * 3), _i([99] * 2), _i([99, 99])
+    paged.page_tables(_i([3, cached]), _i([1, new]), torch.arange(9, dtype=torch.int32, device=DEV), tables, slots, pos, cu,
+                      total, used, page_size=P)
+    assert used[0] == 0 and used.tolist()[1] & paged.TABLE_FULL
+    assert cu.tolist() == [0, 0, 0] and total.tolist() == [3, cached] and slots.tolist() == [-1] * 8
+    assert bool((tables == 7).all())
