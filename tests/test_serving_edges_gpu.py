@@ -298,3 +298,33 @@ def test_lengths_near_2_to_31_are_refused(cached, new):
     assert used[0] == 0 and used.tolist()[1] & paged.TABLE_FULL
     assert cu.tolist() == [0, 0, 0] and total.tolist() == [3, cached] and slots.tolist() == [-1] * 8
     assert bool((tables == 7).all())
+
+
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 32), (16, 4, 128)])
+@pytest.mark.parametrize("new,lens,pre,sizes", [([1, 1], [51, 70], [], []), ([30, 2], [80, 52], [], []),
+                                                ([1, 2, 1], [51, 60, 9], [40, 30], [2, 1]),
+                                                ([20, 9, 1], [70, 59, 51], [300, 90], [2, 1])])
+@pytest.mark.parametrize("where", ["own", "last", "prefix"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_key_that_is_no_number_reaches_what_sees_it(nh, nkv, d, new, lens, pre, sizes, where, value):
+    """One element of one key of kv head 1: the query heads on it become NaN for the tokens that see the key, and every
+    other row is the same bits as without it."""
+    from test_paged_gpu import Batch
+    if where == "prefix" and not pre:
+        return
+    b = Batch(new, lens, nh, nkv, d, 16, pre=pre, sizes=sizes, seed=3)
+    b.q.abs_()  # (an infinite product has one sign: scores of +inf, whose softmax is NaN)
+    clean = b.run()
+    if where == "prefix":
+        b.k[int(b.prefix[0][0, 1]), 1, 3, 5] = value
+        hit = list(range(sum(new[:sizes[0]])))
+    else:
+        at = lens[0] - 1 if where == "last" else 20  # its last key is seen by the last token alone
+        b.k[int(b.tables[0, at // 16]), 1, at % 16, 5] = value
+        hit = [j for j in range(new[0]) if lens[0] - new[0] + j >= at]
+    out = b.run()
+    assert hit and len(hit) < sum(new)
+    o, c = out.view(-1, nkv, nh // nkv * d), clean.view(-1, nkv, nh // nkv * d)
+    assert torch.isnan(o[hit, 1]).all()
+    o[hit, 1] = c[hit, 1]
+    assert torch.equal(o, c)
