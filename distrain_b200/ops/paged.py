@@ -64,7 +64,10 @@ def _fail(msg):
 
 def _launch(name, args, stream):
     """Calls a launcher, which sees for itself what depends on addresses."""
-    rc = _fn(name)(args, stream)
+    rc = (_fns.get(name) or _fn(name))(args, stream)
+    if rc == 0:
+        LAUNCHES[0] += 1
+        return
     if rc == -13:
         _fail(f"{name[3:]}: outputs must not share memory with inputs or each other")
     if rc == -11:
@@ -159,15 +162,14 @@ def page_tables(cached, new, free, tables, slots, positions, cu, total, used, *,
         _fail("free: below 2^31 pages")
     a, b, f, s = cached.data_ptr(), new.data_ptr(), free.data_ptr(), 0 if start is None else start.data_ptr()
     o = (tables.data_ptr(), slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), total.data_ptr(), used.data_ptr())
-    if len({a, b, f, s, *o}) < 10:  # (empty tensors have no address; inputs may be one another)
-        out = [p for p in o if p]
-        if len(set(out)) < len(out) or {a, b, f, s} & set(out):
-            _fail("outputs must not share memory with inputs or each other")
     dev = cached.get_device()
     if not (dev >= 0 and new.get_device() == dev and free.get_device() == dev and tables.get_device() == dev and
             slots.get_device() == dev and positions.get_device() == dev and cu.get_device() == dev and
             total.get_device() == dev and used.get_device() == dev and (start is None or start.get_device() == dev) and
             _current() == dev):
+        out = [p for p in o if p]  # (the launcher looks at every byte, but tensors that are not on a GPU do not get there)
+        if len(set(out)) < len(out) or {a, b, f, s} & set(out):
+            _fail("outputs must not share memory with inputs or each other")
         on_current_device(cached, new, free, tables, slots, positions, cu, total, used, start)
     _launch("dt_page_tables", _TABLES(a, b, s, f, *o, tables.stride(0), n_free, ts[1], n[0], B, shift, 0),
             _stream(stream, dev))
