@@ -875,7 +875,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--rope-theta", type=float)
     p.add_argument("--device", help="torch device for the forward (default cpu)")
-    p.add_argument("--kv-cache", action="store_true", help="compute the prompt once and keep its keys and values (GPU)")
+    p.add_argument("--kv-cache", action="store_true", help="compute the prompt once and keep its keys and values (GPU; logits with more bf16 roundings)")
     p.set_defaults(fn=cmd_generate)
 
     p = sp.add_parser("serve", help="OpenAI-style server for a checkpoint (/v1/completions, /v1/chat/completions)")
@@ -891,7 +891,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-tokens-cap", type=int, default=1024)
     p.add_argument("--rope-theta", type=float)
     p.add_argument("--kv-cache", action="store_true",
-                   help="compute a prompt once, keep its keys and values in pages for all its answers (GPU)")
+                   help="compute a prompt once, keep its keys and values in pages for all its answers (GPU; logits with "
+                        "more bf16 roundings)")
     p.set_defaults(fn=cmd_serve)
 
     p = sp.add_parser("evals", help="multiple-choice benchmark scores of checkpoints (local JSONL task files)")

@@ -7,8 +7,12 @@ and the attention's work list are made on the GPU each step (``ops.paged``); per
 append (bias, rotation, K and V to their slots) and the attention, in which the prompt's keys are read once for all
 answers.
 
-The reference re-runs the whole forward for every new token (node/cli/src/main.rs:1416-1548); this computes the
-same logits from the new tokens alone.
+The reference re-runs the whole forward for every new token (node/cli/src/main.rs:1416-1548); this computes the logits
+from the new tokens alone. They are those of the re-run forward (``serve.EngineLM``) up to roundings, of which there are
+more here: the QKV product is rounded to bf16 before bias and rotation (there, for heads of 64 and 128, the GEMM's
+epilogue adds and rotates its fp32 sums, which for this path would be a GEMM that knows the cache), and the logits are a
+product with the bf16 embedding on the framework's own GEMM (there with the fp32 one). Against the fp32 oracle, with random weights: 9.1e-3
+of the logits' norm off, there 7.9e-3, for the 12-layer preset; 2.0e-2 and 1.7e-2 for the 24-layer one.
 """
 from __future__ import annotations
 
