@@ -13,13 +13,23 @@ inline Span span_rows(const void* p, long long rows, long long bytes, long long 
   return Span{p, stride == 0 && rows > 1 ? 1 : rows, bytes, stride};
 }
 
-// Exact, also for rows that lie in each other's gaps; the search over rows runs only where the whole ranges meet.
+// Exact, also for rows that lie in each other's gaps. Rows are searched only where the whole ranges meet and the strides
+// differ.
 inline bool spans_meet(const Span& x, const Span& y) {
   if (!x.p || !y.p || x.rows <= 0 || y.rows <= 0 || x.bytes <= 0 || y.bytes <= 0) return false;
   const uintptr_t xp = reinterpret_cast<uintptr_t>(x.p), yp = reinterpret_cast<uintptr_t>(y.p);
   if (xp + (x.rows - 1) * x.stride + x.bytes <= yp || yp + (y.rows - 1) * y.stride + y.bytes <= xp) return false;
   const Span &a = x.rows <= y.rows ? x : y, &b = x.rows <= y.rows ? y : x;
   const long long ap = (long long)(reinterpret_cast<uintptr_t>(a.p) - reinterpret_cast<uintptr_t>(b.p));
+  if (a.stride == b.stride && a.bytes <= a.stride && b.bytes <= b.stride) {
+    // row i of a lies `ap + (i - j) * stride` behind row j of b: less than a stride for two neighbouring i - j at most
+    const long long near = -ap / a.stride;
+    for (long long k = near - 1; k <= near + 1; ++k) {
+      const long long at = ap + k * a.stride;
+      if (k > -b.rows && k < a.rows && at < b.bytes && at + a.bytes > 0) return true;
+    }
+    return false;
+  }
   for (long long i = 0; i < a.rows; ++i) {
     const long long from = ap + i * a.stride, to = from + a.bytes;  // relative to b's first row
     // the first row of b that ends behind `from`

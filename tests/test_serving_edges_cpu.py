@@ -96,6 +96,13 @@ def test_spans_meet_where_a_byte_is_in_both():
         assert f(*spans) == want, spans
     assert 4000 < hits < 16000
     assert f(base, 0, 4, 4, base, 1, 4, 4) == 0 and f(base, 1, 0, 0, base, 1, 4, 4) == 0 and f(0, 1, 8, 8, 0, 1, 8, 8) == 0
+    for _ in range(20000):  # rows of one stride, as views of one buffer have
+        stride, spans, sets = rng.randint(6, 20), [], []
+        for _ in range(2):
+            at, rows, nbytes = rng.randint(0, 90), rng.randint(1, 6), rng.randint(1, stride)
+            spans += [base + at, rows, nbytes, stride]
+            sets.append({at + r * stride + i for r in range(rows) for i in range(nbytes)})
+        assert f(*spans) == bool(sets[0] & sets[1]), spans
     far = 1 << 33  # spans past 32 bits
     assert f(base, 2, 4, far, base + far, 1, 4, 4) == 1 and f(base, 2, 4, far, base + far + 4, 1, 4, 4) == 0
 
