@@ -11,8 +11,9 @@ The reference re-runs the whole forward for every new token (node/cli/src/main.r
 from the new tokens alone. They are those of the re-run forward (``serve.EngineLM``) up to roundings, of which there are
 more here: the QKV product is rounded to bf16 before bias and rotation (there, for heads of 64 and 128, the GEMM's
 epilogue adds and rotates its fp32 sums, which for this path would be a GEMM that knows the cache), and the logits are a
-product with the bf16 embedding on the framework's own GEMM (there with the fp32 one). Against the fp32 oracle, with random weights: 9.1e-3
-of the logits' norm off, there 7.9e-3, for the 12-layer preset; 2.0e-2 and 1.7e-2 for the 24-layer one.
+product with the bf16 embedding on the framework's own GEMM (there with the fp32 one). Against the fp32 oracle, with
+random weights, they are 9.1e-3 of their norm off for the 12-layer preset (there 7.9e-3) and 2.0e-2 for the 24-layer one
+(1.7e-2).
 """
 from __future__ import annotations
 

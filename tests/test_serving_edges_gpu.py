@@ -328,3 +328,44 @@ def test_a_key_that_is_no_number_reaches_what_sees_it(nh, nkv, d, new, lens, pre
     assert torch.isnan(o[hit, 1]).all()
     o[hit, 1] = c[hit, 1]
     assert torch.equal(o, c)
+
+
+def test_requests_at_once_and_from_the_command_line(tmp_path, capsys):
+    """HTTP requests that arrive together, on handler threads, give what they give one by one; generate takes a device
+    without an index and refuses a token that the vocabulary does not have."""
+    import concurrent.futures
+    import json
+    import urllib.error
+    import urllib.request
+    from distrain_b200.cli import main
+    from distrain_b200.serve import CompletionServer
+    from distrain_b200.utils.checkpoint import save_safetensors
+    from test_decode_gpu import _decoder
+    _, sd, _ = _decoder(vocab=512)
+    path = str(tmp_path / "m.safetensors")
+    save_safetensors(sd, path)
+    srv = CompletionServer(path, device="cuda", max_tokens_cap=32, kv_cache=True, max_n=4)
+    port = srv.start("127.0.0.1", 0, threads=4)
+
+    def post(body):
+        req = urllib.request.Request(f"http://127.0.0.1:{port}/v1/completions", method="POST", data=json.dumps(body).encode())
+        try:
+            with urllib.request.urlopen(req, timeout=60) as r:
+                return r.status, json.loads(r.read())["choices"]
+        except urllib.error.HTTPError as e:
+            return e.code, None
+    bodies = [{"prompt": [1 + i, 2, 3] * (1 + 20 * i), "max_tokens": 20, "n": 1 + i % 3, "temperature": 0.7 * (i % 2), "seed": i,
+               "presence_penalty": 0.5 * (i // 3)} for i in range(6)]
+    bodies += [{"prompt": [512], "max_tokens": 2}, {"prompt": [1], "max_tokens": 2, "presence_penalty": 1e39}]
+    try:
+        one_by_one = [post(b) for b in bodies]
+        assert [s for s, _ in one_by_one] == [200] * 6 + [400] * 2
+        with concurrent.futures.ThreadPoolExecutor(8) as pool:
+            assert list(pool.map(post, bodies)) == one_by_one
+    finally:
+        srv.stop()
+    main(["generate", path, "--prompt-ids", "5,6,7", "--max-tokens", "4", "--device", "cuda", "--kv-cache"])
+    ids = json.loads(capsys.readouterr().out.strip().splitlines()[-1])["ids"]
+    assert ids[:3] == [5, 6, 7] and len(ids) == 7
+    with pytest.raises(ValueError, match="vocabulary"):
+        main(["generate", path, "--prompt-ids", "5,512", "--max-tokens", "4", "--device", "cuda", "--kv-cache"])
