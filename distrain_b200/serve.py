@@ -88,8 +88,8 @@ class EngineLM:
 
 
 def whole(v) -> int:
-    """``v`` as a whole number; ValueError for a number that is none (1.7, infinity)."""
-    if isinstance(v, float) and not v.is_integer():
+    """``v`` as a whole number; ValueError for what is none (1.7, infinity, true)."""
+    if isinstance(v, bool) or isinstance(v, float) and not v.is_integer():
         raise ValueError(f"{v} is not a whole number")
     return int(v)
 
@@ -124,6 +124,8 @@ class LogitOptions:
             return default if v is None else float(v)
         try:
             allowed = req.get("allowed_token_ids")
+            if not isinstance(allowed, (list, type(None))):  # (the characters of "12" are not what a text means)
+                raise TypeError(f"allowed_token_ids is {type(allowed).__name__}")
             o = cls(number("presence_penalty", 0.0), number("frequency_penalty", 0.0), number("repetition_penalty", 1.0),
                     {whole(k): float(v) for k, v in (req.get("logit_bias") or {}).items()},
                     None if allowed is None else sorted({whole(t) for t in allowed}))

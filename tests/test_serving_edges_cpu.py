@@ -119,3 +119,9 @@ def test_attention_scales_past_the_edge_of_fp32_are_refused(scale):
         paged.paged_attention(*a, scale=scale)
     with pytest.raises(ValueError, match="CUDA"):
         paged.paged_attention(*a, scale=1e-30)
+
+
+@pytest.mark.parametrize("body", [{"allowed_token_ids": "12"}, {"allowed_token_ids": {"5": 1}}, {"allowed_token_ids": [True]},
+                                  {"allowed_token_ids": 7}, {"logit_bias": "7"}])
+def test_fields_of_another_kind_are_refused(srv, body):
+    assert _post(srv, body)[0] == 400
